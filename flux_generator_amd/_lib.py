@@ -61,6 +61,28 @@ class Fp8Mx(C.Structure):      # fluxhip_fp8_mx
                 ("c_mx", c_void_p), ("c_mx_row0", C.c_int32 * 2), ("c_mx_bstride", c_int64), ("c_mx_kstride", c_int64)]
 
 
+class RotaryDesc(C.Structure):      # fluxhip_rotary_desc
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+                ("q_strides", c_int64 * 3), ("k_strides", c_int64 * 3), ("qo_strides", c_int64 * 3), ("ko_strides", c_int64 * 3),
+                ("positions", c_void_p), ("freqs", c_void_p), ("pos_strides", c_int64 * 2), ("B", c_int64), ("T", c_int64),
+                ("H", C.c_int32), ("K", C.c_int32), ("hd", C.c_int32), ("rot", C.c_int32), ("interleaved", C.c_int32),
+                ("inverse", C.c_int32), ("pos64", C.c_int32), ("n_axes", C.c_int32), ("axis_pairs", C.c_int32 * 4),
+                ("dtype", C.c_int32), ("scale", c_float)]
+
+
+class GatedFfDesc(C.Structure):      # fluxhip_gated_ff_desc
+    _fields_ = [(n, c_void_p) for n in ("x", "w_value", "w_gate", "w_out", "b_value", "b_gate", "b_out", "value", "gate", "hidden", "y")] + [
+        ("M", c_int64), ("ldx", c_int64), ("D", C.c_int32), ("F", C.c_int32), ("act", C.c_int32), ("dtype", C.c_int32),
+        ("ws", c_void_p), ("ws_bytes", c_int64)]
+
+
+class GatedFfGradDesc(C.Structure):      # fluxhip_gated_ff_grad_desc
+    _fields_ = [(n, c_void_p) for n in ("dy", "x", "value", "gate", "hidden", "w_value", "w_gate", "w_out", "dvalue", "dgate", "dx",
+                                        "dw_value", "dw_gate", "dw_out", "db_value", "db_gate", "db_out")] + [
+        ("M", c_int64), ("ldx", c_int64), ("lddy", c_int64), ("D", C.c_int32), ("F", C.c_int32), ("act", C.c_int32),
+        ("dtype", C.c_int32), ("ws", c_void_p), ("ws_bytes", c_int64)]
+
+
 # name -> (restype, argtypes); every symbol include/fluxhip.h declares
 SIGNATURES = {
     "fluxhip_abi_version": (c_int, []),
@@ -150,6 +172,18 @@ SIGNATURES = {
     "fluxhip_embedding_x3": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
     "fluxhip_pixel_linear_x3_f32in": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
                                               c_float, c_void_p]),
+    # forward with what the gradient needs, and the gradient (adapter training)
+    "fluxhip_layernorm_stats": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p,
+                                        c_void_p, c_int64, c_int64, c_int, c_float, c_int, c_void_p]),
+    "fluxhip_layernorm_grad_ws": (c_int64, [c_int64, c_int64, c_int]),
+    "fluxhip_layernorm_grad": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+                                       c_int, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p,
+                                       c_int64, c_void_p]),
+    "fluxhip_rotary": (c_int, [C.POINTER(RotaryDesc), c_void_p]),
+    "fluxhip_gated_ff_ws": (c_int64, [c_int64, c_int, c_int]),
+    "fluxhip_gated_ff": (c_int, [C.POINTER(GatedFfDesc), c_void_p]),
+    "fluxhip_gated_ff_grad_ws": (c_int64, [c_int64, c_int, c_int]),
+    "fluxhip_gated_ff_grad": (c_int, [C.POINTER(GatedFfGradDesc), c_void_p]),
 }
 # float16-storage twins (the stable_diffusion/ models with float16=True): same signatures as the bf16 entry points
 for _b, _f in (("fluxhip_gemm_bf16", "fluxhip_gemm_f16"), ("fluxhip_conv2d_bf16", "fluxhip_conv2d_f16"),

@@ -1,0 +1,66 @@
+// Element types of the operators that take bfloat16, float16 or float32 tensors (dtype codes of include/fluxhip.h): 8-element
+// chunks to and from float32 registers.  Rows need element alignment only; a chunk that a row's end cuts is moved by element.
+#pragma once
+#include "common.h"
+
+template <int T> struct Elem;
+
+template <bool H>
+struct Elem16 {
+  typedef uint16_t type;
+  static DEVINL float get(const type* p) { return e2f<H>(*p); }
+  static DEVINL void put(type* p, float v) { *p = f2e<H>(v); }
+  static DEVINL void load8(const type* p, int c, int n, float (&v)[8]) {
+    if (c + 8 <= n) {
+      uint32_t w[4];
+      __builtin_memcpy(w, p + c, 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = e_lo<H>(w[j]);
+        v[2 * j + 1] = e_hi<H>(w[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < n ? e2f<H>(p[c + j]) : 0.f;
+    }
+  }
+  static DEVINL void store8(type* p, int c, int n, const float (&v)[8]) {
+    if (c + 8 <= n) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = e_pack<H>(v[2 * j], v[2 * j + 1]);
+      __builtin_memcpy(p + c, w, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < n) p[c + j] = f2e<H>(v[j]);
+    }
+  }
+};
+template <> struct Elem<0> : Elem16<false> {};
+template <> struct Elem<1> : Elem16<true> {};
+template <>
+struct Elem<2> {
+  typedef float type;
+  static DEVINL float get(const type* p) { return *p; }
+  static DEVINL void put(type* p, float v) { *p = v; }
+  static DEVINL void load8(const float* p, int c, int n, float (&v)[8]) {
+    if (c + 8 <= n) {
+      __builtin_memcpy(&v[0], p + c, 16);
+      __builtin_memcpy(&v[4], p + c + 4, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < n ? p[c + j] : 0.f;
+    }
+  }
+  static DEVINL void store8(float* p, int c, int n, const float (&v)[8]) {
+    if (c + 8 <= n) {
+      __builtin_memcpy(p + c, &v[0], 16);
+      __builtin_memcpy(p + c + 4, &v[4], 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < n) p[c + j] = v[j];
+    }
+  }
+};

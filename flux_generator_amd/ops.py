@@ -6,12 +6,13 @@ hand-written gfx950 kernel launched through ctypes.  All tensors must be CUDA(HI
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
-from ._lib import Fp8Mx, Fp8Scales, GemmDesc, GemmX3Desc
+from ._lib import Fp8Mx, Fp8Scales, GatedFfDesc, GatedFfGradDesc, GemmDesc, GemmX3Desc, RotaryDesc
 
 EPI_BIAS, EPI_GELU_TANH, EPI_GATE_RES, EPI_SPLIT_GELU, EPI_SILU, EPI_GEGLU, EPI_QUICK_GELU, EPI_GELU_ERF, EPI_GEGLU_PAIR = 0, 1, 2, 3, 4, 5, 6, 7, 8
 BF16 = torch.bfloat16
@@ -944,3 +945,333 @@ def attention_x3(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, H: int, Tk:
         gemm_x3_batched(pm, vt[:, b0:b0 + n], o_hm, N, 64, Tkpad, Tkpad, 64, n * H, N * Tkpad, 64 * Tkpad, N * 64)
         o[:, b0:b0 + n].copy_(o_hm.permute(0, 1, 3, 2, 4).reshape(2, n, N, C))
     return o
+
+
+# ------------------------------------------------------------------------------------------------ adapter training: operators of a
+# transformer block outside attention, forward (returning what the gradient needs) and backward.  No state is kept here: scratch
+# memory is allocated per call from torch's allocator (of the capturing graph's own pool inside a capture).
+_DT = {BF16: 0, F16: 1, F32: 2}
+
+
+def _on_device(*named) -> None:
+    """Every given (tensor, name) pair lives on the current device, whose stream the launch goes to."""
+    dev = None
+    for t, name in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise FluxHipError("libfluxhip ops need device tensors (no CPU fallback exists)")
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if t.get_device() != dev:
+            raise FluxHipError(f"{name} is on {t.device}, the current device is cuda:{dev} (one process drives one GPU)")
+
+
+def _samples(t: torch.Tensor, name: str, per_sample: bool):
+    """(B, T, sample stride, row stride) of a [..., D] tensor with a contiguous last dimension; per_sample: B is its first dimension."""
+    if t.dim() < 1 or t.shape[-1] < 1 or (t.stride(-1) != 1 and t.shape[-1] != 1):
+        raise FluxHipError(f"{name} must be [..., D] with a contiguous last dimension")
+    shape, st, D = t.shape, t.stride(), t.shape[-1]
+    if t.is_contiguous():
+        rows = t.numel() // D
+        if not per_sample:
+            return 1, rows, 0, D
+        return shape[0], rows // max(1, shape[0]), rows // max(1, shape[0]) * D, D
+    lo = 1 if per_sample else 0                      # rows = dims lo .. -2 as one run, or (without per_sample) dims 1 .. -2 and dim 0 apart
+    run = [i for i in range(t.dim() - 1) if i >= lo and shape[i] != 1]
+    if not per_sample and len(run) > 1 and any(st[a] != st[b] * shape[b] for a, b in zip(run, run[1:])):
+        lo, run = 1, [i for i in run if i >= 1]
+    if any(st[a] != st[b] * shape[b] for a, b in zip(run, run[1:])):
+        raise FluxHipError(f"{name}: the rows of a sample must lie at one stride")
+    T = 1
+    for i in run:
+        T *= shape[i]
+    return (shape[0] if lo else 1), T, (st[0] if lo else 0), (st[run[-1]] if run else D)
+
+
+def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, name: str):
+    """(per sample?, float32?) of a LayerNorm parameter: [D] or [B, D], x's type or float32."""
+    if p is None:
+        return None
+    D = x.shape[-1]
+    if p.dtype not in (x.dtype, F32) or not p.is_contiguous():
+        raise FluxHipError(f"{name} must be a contiguous tensor of x's type or float32")
+    if tuple(p.shape) == (D,):
+        return False, p.dtype == F32 and x.dtype != F32
+    if x.dim() >= 2 and tuple(p.shape) == (x.shape[0], D):
+        return True, p.dtype == F32 and x.dtype != F32
+    raise FluxHipError(f"{name} must be [{D}] or [{x.shape[0] if x.dim() >= 2 else 1}, {D}], not {list(p.shape)}")
+
+
+def _norm_args(x, gamma, beta, other=None):
+    if x.dtype not in _DT:
+        raise FluxHipError("x must be bfloat16, float16 or float32")
+    if gamma is None and beta is not None:
+        raise FluxHipError("beta needs gamma")
+    g, b = _norm_param(gamma, x, "gamma"), _norm_param(beta, x, "beta")
+    if g is not None and b is not None and (g != b or gamma.dtype != beta.dtype):
+        raise FluxHipError("gamma and beta must have one shape and one type")
+    per, pf = g if g is not None else (False, False)
+    if per and x.shape[0] > 65535:
+        raise FluxHipError("per-sample parameters: at most 65535 samples")
+    xs = _samples(x, "x", per)
+    if other is not None:
+        if other.shape != x.shape or other.dtype != x.dtype:
+            raise FluxHipError("dy must have x's shape and type")
+        os_ = _samples(other, "dy", per)
+        if os_[:2] != xs[:2]:                        # one is a view of separate samples, the other one run of rows
+            B = x.shape[0]
+            split = lambda s, t: s if s[0] == B and B > 1 else (B, s[1] // B, s[1] // B * s[3], s[3])
+            xs, os_ = split(xs, x), split(os_, other)
+        return per, pf, xs, os_
+    if xs[0] > 65535:
+        raise FluxHipError("x: at most 65535 separately strided samples")
+    return per, pf, xs, None
+
+
+def layernorm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None, eps: float = 1e-5,
+              unit_offset: bool = False):
+    """LayerNorm over the last dimension with the statistics `layernorm_backward` needs: (y, mean, rstd), mean / rstd float32
+    [x.shape[:-1]].  x [..., D] bf16 / f16 / f32, any D, rows at one stride inside a sample (slices of packed buffers work).
+    gamma, beta: [D], or one vector per sample [x.shape[0], D] (adaLN); unit_offset multiplies by 1 + gamma."""
+    per, pf, (B, T, bs, rs), _ = _norm_args(x, gamma, beta)
+    _on_device((x, "x"), (gamma, "gamma"), (beta, "beta"))
+    D = x.shape[-1]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(x.shape[:-1], dtype=F32, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=F32, device=x.device)
+    _check(_lib.load().fluxhip_layernorm_stats(x.data_ptr(), bs, rs, _p(gamma), _p(beta), D if per else 0, int(pf),
+                                               1.0 if unit_offset else 0.0, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), B, T, D,
+                                               eps, _DT[x.dtype], _stream()), "fluxhip_layernorm_stats")
+    return y, mean, rstd
+
+
+def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                       gamma: Optional[torch.Tensor] = None, unit_offset: bool = False, param_grads: bool = True):
+    """Gradient of `layernorm`: (dx, dgamma, dbeta).  dgamma / dbeta have gamma's shape and type (their sums run in float32 in a
+    fixed order); None without gamma or with param_grads=False (frozen norms)."""
+    per, pf, (B, T, bs, rs), (_, _, dbs, drs) = _norm_args(x, gamma, None, dy)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype != F32 or not t.is_contiguous() or t.shape != x.shape[:-1]:
+            raise FluxHipError(f"{name} must be the contiguous float32 [{', '.join(map(str, x.shape[:-1]))}] of layernorm")
+    _on_device((x, "x"), (dy, "dy"), (gamma, "gamma"), (mean, "mean"), (rstd, "rstd"))
+    lib, D = _lib.load(), x.shape[-1]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dg = db = ws = None
+    n = 0
+    if gamma is not None and param_grads:
+        if x.numel() == 0:
+            return dx, torch.zeros_like(gamma), torch.zeros_like(gamma)
+        dg, db = torch.empty_like(gamma), torch.empty_like(gamma)
+        n = lib.fluxhip_layernorm_grad_ws(B, T, D)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    _check(lib.fluxhip_layernorm_grad(dy.data_ptr(), dbs, drs, x.data_ptr(), bs, rs, mean.data_ptr(), rstd.data_ptr(), _p(gamma),
+                                      D if per else 0, int(pf), 1.0 if unit_offset else 0.0, dx.data_ptr(), _p(dg), _p(db), B, T, D,
+                                      _DT[x.dtype], _p(ws), n, _stream()), "fluxhip_layernorm_grad")
+    return dx, dg, db
+
+
+def rotary_frequencies(dims, theta: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0, original_length: int = 0,
+                       beta_fast: float = 32.0, beta_slow: float = 1.0, device="cuda"):
+    """(freqs float64 [sum(dims) / 2], scale) for `rotary`: theta^(-2 j / d) over the pairs of every axis width d in `dims` (an int:
+    one axis).  For contexts `factor` times the trained length:  "linear" divides every frequency by factor;  "ntk" raises theta to
+    theta factor^(d / (d - 2)), which leaves the fastest pair and divides the slowest by factor;  "yarn" divides the pairs that
+    turn fewer than beta_slow times over original_length positions, keeps those above beta_fast, blends linearly (in the pair index)
+    between, and scales by 0.1 ln(factor) + 1."""
+    dims = [dims] if isinstance(dims, int) else list(dims)
+    if not dims or any(d < 2 or d % 2 for d in dims):
+        raise FluxHipError("rotary widths must be even and at least 2")
+    if scaling not in (None, "linear", "ntk", "yarn") or factor < 1.0 or theta <= 0.0:
+        raise FluxHipError("scaling must be None, 'linear', 'ntk' or 'yarn', with factor >= 1 and theta > 0")
+    if scaling == "yarn" and (original_length < 1 or not beta_fast > beta_slow > 0):
+        raise FluxHipError("yarn needs original_length >= 1 and beta_fast > beta_slow > 0")
+    parts = []
+    for d in dims:
+        j = torch.arange(0, d, 2, dtype=torch.float64)
+        base = theta
+        if scaling == "ntk" and d > 2:
+            base = theta * factor ** (d / (d - 2))
+        f = base ** (-j / d)
+        if scaling == "linear":
+            f = f / factor
+        elif scaling == "yarn":
+            pair = lambda turns: d * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+            lo, hi = max(0, math.floor(pair(beta_fast))), min(d // 2 - 1, math.ceil(pair(beta_slow)))
+            keep = 1 - ((j / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+            f = f * keep + f / factor * (1 - keep)
+        parts.append(f)
+    scale = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" and factor > 1.0 else 1.0
+    return torch.cat(parts).to(device), scale
+
+
+def _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, inverse, out):
+    if q.dim() != 4 or q.dtype not in _DT:
+        raise FluxHipError("q must be [B, T, H, head_dim] of bfloat16, float16 or float32")
+    B, T, H, hd = q.shape
+    if k is not None and (k.dim() != 4 or k.shape[0] != B or k.shape[1] != T or k.shape[3] != hd or k.dtype != q.dtype):
+        raise FluxHipError("k must be [B, T, K, head_dim] with q's B, T, head_dim and type")
+    if freqs.dim() != 1 or freqs.dtype != torch.float64 or not freqs.is_contiguous():
+        raise FluxHipError("freqs must be the contiguous float64 [rot / 2] of rotary_frequencies")
+    rot = 2 * freqs.shape[0]
+    dims = [rot] if axes_dim is None else list(axes_dim)
+    if rot < 2 or rot > hd or len(dims) > 4 or any(d < 0 or d % 2 for d in dims) or sum(dims) != rot:
+        raise FluxHipError("rot = 2 len(freqs) must be in [2, head_dim] and the sum of at most 4 even axes_dim")
+    na = len(dims)
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise FluxHipError("positions must be int32 or int64")
+    lead = (T,) if na == 1 else (T, na)
+    if tuple(positions.shape) not in (lead, (B,) + lead) or (na > 1 and positions.stride(-1) != 1):
+        raise FluxHipError(f"positions must be [T] or [B, T]{', with the axes last and contiguous' if na > 1 else ''}")
+    ps = positions.stride()
+    pb = ps[0] if positions.dim() == len(lead) + 1 else 0
+    pt = ps[-1] if na == 1 else ps[-2]
+    outs = [None, None] if out is None else ([out, None] if isinstance(out, torch.Tensor) else list(out))
+    if len(outs) != 2 or (k is None and outs[1] is not None) or (out is not None and k is not None and outs[1] is None):
+        raise FluxHipError("out must give one tensor for each of q and k")
+    d = RotaryDesc()
+    got = []
+    for t, o, name in ((q, outs[0], "q"), (k, outs[1], "k")):
+        if t is None:
+            continue
+        if t.stride(-1) != 1 and hd != 1:
+            raise FluxHipError(f"{name} must have a contiguous last dimension")
+        if o is None:
+            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        elif o.shape != t.shape or o.dtype != t.dtype or o.stride(-1) != 1:
+            raise FluxHipError(f"out must have {name}'s shape and type and a contiguous last dimension")
+        got.append(o)
+        s, so = t.stride(), o.stride()
+        if any(so[i] == 0 and t.shape[i] > 1 for i in range(3)):
+            raise FluxHipError("out must not be a broadcast view")
+        if name == "q":
+            d.q_strides[:], d.qo_strides[:] = s[:3], so[:3]
+        else:
+            d.k_strides[:], d.ko_strides[:] = s[:3], so[:3]
+    _on_device((q, "q"), (k, "k"), (positions, "positions"), (freqs, "freqs"), *((o, "out") for o in got))
+    d.q, d.q_out = q.data_ptr(), got[0].data_ptr()
+    if k is not None:
+        d.k, d.k_out, d.K = k.data_ptr(), got[1].data_ptr(), k.shape[2]
+    d.positions, d.freqs, d.pos64 = positions.data_ptr(), freqs.data_ptr(), positions.dtype == torch.int64
+    d.pos_strides[:] = (pb, pt)
+    d.B, d.T, d.H, d.hd, d.rot, d.n_axes = B, T, H, hd, rot, na
+    d.axis_pairs[:na] = [w // 2 for w in dims]
+    d.interleaved, d.inverse, d.dtype, d.scale = interleaved, inverse, _DT[q.dtype], scale
+    _check(_lib.load().fluxhip_rotary(ctypes.byref(d), _stream()), "fluxhip_rotary")
+    return got[0] if k is None else (got[0], got[1])
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, axes_dim=None,
+           interleaved: bool = True, scale: float = 1.0, out=None):
+    """Rotary positions on q [B, T, H, head_dim] and k [B, T, K, head_dim] (or None) in one launch -> (q', k') (or q').  Any strides
+    with a contiguous last dimension (transposed heads, slices of a fused projection); out: tensors to write, which may be the
+    inputs themselves.  positions [T] or [B, T] integers, with axes_dim of several axes [T, axes] or [B, T, axes]; freqs, scale:
+    rotary_frequencies.  The first 2 len(freqs) columns turn - pairs (2j, 2j + 1) when interleaved, else (j, j + half) -, the rest is
+    copied.  Angles are formed in 64 bits."""
+    return _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, False, out)
+
+
+def rotary_backward(dq: torch.Tensor, dk: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, axes_dim=None,
+                    interleaved: bool = True, scale: float = 1.0, out=None):
+    """Gradient of `rotary`: the turn by the negative angles with the same scale."""
+    return _rotary(dq, dk, positions, freqs, axes_dim, interleaved, scale, True, out)
+
+
+_FF_ACTS = (EPI_GELU_TANH, EPI_GELU_ERF, EPI_SILU)
+
+
+def _ff_rows(t: torch.Tensor, name: str, D: int, dtype) -> tuple:
+    """(rows, row stride) of a [..., D] operand of the gated feed-forward."""
+    if t.dtype != dtype or t.dim() < 1 or t.shape[-1] != D:
+        raise FluxHipError(f"{name} must be [..., {D}] of {dtype}")
+    B, M, bs, ld = _samples(t, name, False)
+    if B > 1:
+        raise FluxHipError(f"{name}: the rows must lie at one stride")
+    ld = D if M <= 1 else ld
+    if ld < D or ld % 8 or t.data_ptr() % 16:
+        raise FluxHipError(f"{name}: rows must be 16-byte aligned, a multiple of 8 elements apart and not overlap")
+    return B * M, ld
+
+
+def _ff_weights(x, w_value, w_gate, w_out, act):
+    if x.dtype not in (BF16, F16):
+        raise FluxHipError("x must be bfloat16 or float16")
+    if act not in _FF_ACTS:
+        raise FluxHipError("act must be EPI_GELU_TANH, EPI_GELU_ERF or EPI_SILU")
+    if w_value.dim() != 2:
+        raise FluxHipError("w_value must be [F, D]")
+    F, D = w_value.shape
+    if D < 8 or F < 8 or D % 8 or F % 8:
+        raise FluxHipError("gated_ff needs widths that are multiples of 8")
+    for t, name, shape in ((w_value, "w_value", (F, D)), (w_gate, "w_gate", (F, D)), (w_out, "w_out", (D, F))):
+        if tuple(t.shape) != shape or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16:
+            raise FluxHipError(f"{name} must be a contiguous, 16-byte aligned {list(shape)} tensor of {x.dtype}")
+    return D, F
+
+
+def gated_ff(x: torch.Tensor, w_value: torch.Tensor, w_gate: torch.Tensor, w_out: torch.Tensor, b_value: Optional[torch.Tensor] = None,
+             b_gate: Optional[torch.Tensor] = None, b_out: Optional[torch.Tensor] = None, act: int = EPI_GELU_ERF, save: bool = False):
+    """y = ((x Wv^T + bv) * act(x Wg^T + bg)) Wo^T + bo for x [..., D], w_value / w_gate [F, D], w_out [D, F] (bf16 or f16, D and F
+    multiples of 8): both projections, the activation and the product are one kernel, w_out's product the other.  save: returns
+    (y, (value, gate, hidden)) for `gated_ff_backward`."""
+    D, F = _ff_weights(x, w_value, w_gate, w_out, act)
+    M, ldx = _ff_rows(x, "x", D, x.dtype)
+    if (b_value is None) != (b_gate is None):
+        raise FluxHipError("b_value and b_gate go together")
+    for t, name, n in ((b_value, "b_value", F), (b_gate, "b_gate", F), (b_out, "b_out", D)):
+        if t is not None and (tuple(t.shape) != (n,) or t.dtype != x.dtype or not t.is_contiguous()):
+            raise FluxHipError(f"{name} must be a contiguous [{n}] tensor of {x.dtype}")
+    _on_device((x, "x"), (w_value, "w_value"), (w_gate, "w_gate"), (w_out, "w_out"), (b_value, "b_value"), (b_gate, "b_gate"), (b_out, "b_out"))
+    lib, lead = _lib.load(), x.shape[:-1]
+    y = torch.empty(*lead, D, dtype=x.dtype, device=x.device)
+    hidden = torch.empty(*lead, F, dtype=x.dtype, device=x.device)
+    saved = (torch.empty_like(hidden), torch.empty_like(hidden), hidden) if save else None
+    d = GatedFfDesc()
+    n = lib.fluxhip_gated_ff_ws(M, D, F)
+    if n > 0:
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        d.ws, d.ws_bytes = ws.data_ptr(), n
+    d.x, d.w_value, d.w_gate, d.w_out, d.hidden, d.y = (t.data_ptr() for t in (x, w_value, w_gate, w_out, hidden, y))
+    d.b_value, d.b_gate, d.b_out = _p(b_value), _p(b_gate), _p(b_out)
+    if save:
+        d.value, d.gate = saved[0].data_ptr(), saved[1].data_ptr()
+    d.M, d.ldx, d.D, d.F, d.act, d.dtype = M, ldx, D, F, act, _DT[x.dtype]
+    _check(lib.fluxhip_gated_ff(ctypes.byref(d), _stream()), "fluxhip_gated_ff")
+    return (y, saved) if save else y
+
+
+def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, saved, w_value: torch.Tensor, w_gate: torch.Tensor, w_out: torch.Tensor,
+                      act: int = EPI_GELU_ERF, input_grad: bool = True, weight_grads: bool = True, bias_grads: bool = False):
+    """Gradient of `gated_ff` from its saved (value, gate, hidden): (dx, dw_value, dw_gate, dw_out, db_value, db_gate, db_out), None
+    where not asked for (weight_grads=False: adapter training on frozen weights, half the work)."""
+    D, F = _ff_weights(x, w_value, w_gate, w_out, act)
+    M, ldx = _ff_rows(x, "x", D, x.dtype)
+    if dy.shape != x.shape:
+        raise FluxHipError("dy must have x's shape")
+    _, lddy = _ff_rows(dy, "dy", D, x.dtype)
+    value, gate, hidden = saved
+    for t, name in ((value, "value"), (gate, "gate"), (hidden, "hidden")):
+        if t.shape != (*x.shape[:-1], F) or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16:
+            raise FluxHipError(f"{name} must be the contiguous [..., {F}] tensor gated_ff saved")
+    _on_device((x, "x"), (dy, "dy"), (value, "value"), (gate, "gate"), (hidden, "hidden"), (w_value, "w_value"), (w_gate, "w_gate"),
+               (w_out, "w_out"))
+    lib = _lib.load()
+    new = lambda t: torch.empty(t.shape, dtype=x.dtype, device=x.device)
+    dx = new(x) if input_grad else None
+    dw = [new(w) for w in (w_value, w_gate, w_out)] if weight_grads else [None] * 3
+    db = [torch.empty(n, dtype=x.dtype, device=x.device) for n in (F, F, D)] if bias_grads else [None] * 3
+    if M == 0:
+        for t in dw + db:
+            if t is not None:
+                t.zero_()
+        return (dx, *dw, *db)
+    dvalue, dgate = new(value), new(value)
+    d = GatedFfGradDesc()
+    n = lib.fluxhip_gated_ff_grad_ws(M, D, F)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    d.ws, d.ws_bytes = ws.data_ptr(), n
+    d.dy, d.x, d.value, d.gate, d.hidden = (t.data_ptr() for t in (dy, x, value, gate, hidden))
+    d.w_value, d.w_gate, d.w_out, d.dvalue, d.dgate = (t.data_ptr() for t in (w_value, w_gate, w_out, dvalue, dgate))
+    d.dx, d.dw_value, d.dw_gate, d.dw_out, d.db_value, d.db_gate, d.db_out = (_p(t) for t in (dx, *dw, *db))
+    d.M, d.ldx, d.lddy, d.D, d.F, d.act, d.dtype = M, ldx, lddy, D, F, act, _DT[x.dtype]
+    _check(lib.fluxhip_gated_ff_grad(ctypes.byref(d), _stream()), "fluxhip_gated_ff_grad")
+    return (dx, *dw, *db)

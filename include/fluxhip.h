@@ -523,6 +523,83 @@ int fluxhip_embedding_x3(const int* idx, const float* table, const float* pos, v
 int fluxhip_pixel_linear_x3_f32in(const float* x, const float* w, const float* bias, void* out, int64_t out_lo, int64_t npix,
                                   int Cin, int Cout, int Cpad, float in_div, void* stream);
 
+/* ---- forward with what the gradient needs, and the gradient: training adapters through the transformer blocks --------
+ * The reference fine-tunes adapters with its framework's automatic differentiation (dreambooth.py:193-230); these are the
+ * operators of a transformer block outside attention, forward and backward.  Nothing here keeps state: statistics, saved
+ * activations and scratch memory are the caller's, work is enqueued on `stream`, results do not depend on the run (no
+ * atomics).  Rows need element alignment only unless said otherwise. */
+enum { FLUXHIP_DT_BF16 = 0, FLUXHIP_DT_F16 = 1, FLUXHIP_DT_F32 = 2 };
+
+/* y = (x - mean) rstd (offset + gamma) + beta over rows of width D, with mean and rstd = 1 / sqrt(var + eps) float32 per row.
+ * B samples of T rows; row (b, t) of x at x + b x_bs + t x_rs (elements), y and the statistics contiguous.  gamma / beta: [D]
+ * (p_bs = 0) or one vector per sample (p_bs elements apart; adaLN with offset = 1, flux/layers.py:192-193); float32 if
+ * param_f32, else x's type; both NULL or beta alone NULL allowed (offset is then not applied without gamma). */
+int fluxhip_layernorm_stats(const void* x, int64_t x_bs, int64_t x_rs, const void* gamma, const void* beta, int64_t p_bs,
+                            int param_f32, float offset, void* y, float* mean, float* rstd, int64_t B, int64_t T, int D,
+                            float eps, int dtype, void* stream);
+/* Its gradient: dx [B][T][D] contiguous, and (both or neither) dgamma, dbeta shaped and typed like the parameters ([D], or
+ * [B][D] contiguous when p_bs != 0).  ws: fluxhip_layernorm_grad_ws bytes of scratch when the parameter gradients are asked
+ * for.  An empty x (B or T zero) writes nothing. */
+int64_t fluxhip_layernorm_grad_ws(int64_t B, int64_t T, int D);
+int fluxhip_layernorm_grad(const void* dy, int64_t dy_bs, int64_t dy_rs, const void* x, int64_t x_bs, int64_t x_rs,
+                           const float* mean, const float* rstd, const void* gamma, int64_t p_bs, int param_f32, float offset,
+                           void* dx, void* dgamma, void* dbeta, int64_t B, int64_t T, int D, int dtype, void* ws,
+                           int64_t ws_bytes, void* stream);
+
+/* Rotary positions on q [B][T][H][hd] and k [B][T][K][hd] (element strides of batch, token, head; the last dimension is
+ * contiguous; out may be in).  Pair j < rot / 2 of a token turns by positions[.., axis(j)] * freqs[j] (formed in 64 bits) and is
+ * scaled by `scale`; columns >= rot are copied.  interleaved: pairs (2j, 2j + 1), else (j, j + rot / 2).  Axis i owns
+ * axis_pairs[i] consecutive pairs (their sum is rot / 2).  inverse: the turn by the negative angle = the gradient.
+ * flux/layers.py:29-33,60-75 in general form. */
+typedef struct fluxhip_rotary_desc {
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t q_strides[3], k_strides[3], qo_strides[3], ko_strides[3];
+  const void* positions;   /* int32 or int64 (pos64) [B][T][n_axes], element strides of batch and token        */
+  const void* freqs;       /* float64 [rot / 2], radians per position                                          */
+  int64_t pos_strides[2];
+  int64_t B, T;
+  int32_t H, K, hd, rot;
+  int32_t interleaved, inverse, pos64, n_axes;
+  int32_t axis_pairs[4];
+  int32_t dtype;           /* FLUXHIP_DT_*                                                                     */
+  float scale;
+} fluxhip_rotary_desc;
+int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream);
+
+/* Gated feed-forward block: value = x Wv^T + bv, gate = x Wg^T + bg, hidden = value act(gate), y = hidden Wo^T + bo
+ * (stable_diffusion/.../unet.py:74-78 and its linear3; flux/t5.py:163-177).  Weights [F][D], [F][D], [D][F] row-major, D % 8 == 0,
+ * F % 8 == 0, every pointer 16-byte aligned, ldx % 8 == 0.  act: FLUXHIP_EPI_GELU_TANH, FLUXHIP_EPI_GELU_ERF or
+ * FLUXHIP_EPI_SILU.  dtype: bf16 or f16; products accumulate in float32; value, gate and hidden are rounded to dtype (hidden is
+ * formed from the unrounded two).  value / gate may be NULL (both); hidden [M][F] is always written. */
+typedef struct fluxhip_gated_ff_desc {
+  const void *x, *w_value, *w_gate, *w_out;
+  const void *b_value, *b_gate, *b_out;      /* bv and bg both or neither                              */
+  void *value, *gate, *hidden, *y;           /* [M][F] x 3, [M][D], contiguous                         */
+  int64_t M, ldx;
+  int32_t D, F, act, dtype;
+  void* ws;                                  /* fluxhip_gated_ff_ws bytes                              */
+  int64_t ws_bytes;
+} fluxhip_gated_ff_desc;
+int64_t fluxhip_gated_ff_ws(int64_t M, int D, int F);
+int fluxhip_gated_ff(const fluxhip_gated_ff_desc* d, void* stream);
+
+/* Its gradient from dy and the saved value, gate (and hidden, for dw_out):
+ *   dh = dy Wo, dvalue = dh act(gate), dgate = dh value act'(gate)   (rounded to dtype, [M][F] each, written for the products below)
+ *   dx = dvalue Wv + dgate Wg, dWv = dvalue^T x, dWg = dgate^T x, dWo = dy^T hidden, db = column sums (of the unrounded values).
+ * Outputs that are NULL are not computed (dw_value and dw_gate together, the three db together).  ldx, lddy % 8 == 0. */
+typedef struct fluxhip_gated_ff_grad_desc {
+  const void *dy, *x, *value, *gate, *hidden, *w_value, *w_gate, *w_out;
+  void *dvalue, *dgate;
+  void *dx, *dw_value, *dw_gate, *dw_out, *db_value, *db_gate, *db_out;
+  int64_t M, ldx, lddy;
+  int32_t D, F, act, dtype;
+  void* ws;                                  /* fluxhip_gated_ff_grad_ws bytes                         */
+  int64_t ws_bytes;
+} fluxhip_gated_ff_grad_desc;
+int64_t fluxhip_gated_ff_grad_ws(int64_t M, int D, int F);
+int fluxhip_gated_ff_grad(const fluxhip_gated_ff_grad_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
