@@ -14,6 +14,7 @@
 #include "elem.h"
 #include "colsum.h"
 
+
 namespace {
 
 struct LnArgs {
@@ -26,66 +27,89 @@ struct LnArgs {
   float eps, offset;
 };
 
-// sum over the WPR waves that share a row; red: two slots of 4 floats, used in turn (a slot is rewritten only behind the next
-// barrier, which every reader of it has passed)
-template <int WPR>
-DEVINL float row_sum(float v, float (*red)[4], int& turn) {
+// blocks of eight waves: 8 / WPR rows side by side, WPR waves a row
+constexpr int WAVES = 8;
+
+// sums (one or two at once) over the WPR waves that share a row; red: two slots, used in turn (a slot is rewritten only behind
+// the next barrier, which every reader of it has passed)
+DEVINL float wave_total(float v) {
   v = row16_sum(v);
   const int i = __builtin_bit_cast(int, v);
-  v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16)) +
-      __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 48));
-  if constexpr (WPR == 1) return v;
-  const int s = turn;
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16)) +
+         __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 48));
+}
+template <int WPR>
+DEVINL float2 row_sum2(float a, float b, float2 (*red)[WAVES], int& turn) {
+  a = wave_total(a);
+  b = wave_total(b);
+  if constexpr (WPR == 1) return make_float2(a, b);
+  const int s = turn, w = threadIdx.x >> 6, w0 = w & ~(WPR - 1);
   turn ^= 1;
-  if ((threadIdx.x & 63) == 0) red[s][threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) red[s][w] = make_float2(a, b);
   __syncthreads();
-  return red[s][0] + red[s][1] + red[s][2] + red[s][3];
+  float2 r = red[s][w0];
+#pragma unroll
+  for (int i = 1; i < WPR; ++i) {
+    r.x += red[s][w0 + i].x;
+    r.y += red[s][w0 + i].y;
+  }
+  return r;
 }
 
-template <int T, int NCH, int NT>
-DEVINL void load_row(const typename Elem<T>::type* p, int tr, int D, float (&v)[NCH][8]) {
+template <int T, int NCH, int NT, bool FULL>
+DEVINL void fetch_row(const typename Elem<T>::type* p, int tr, int D, typename Elem<T>::raw8 (&w)[NCH]) {
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) Elem<T>::load8(p, (tr + i * NT) * 8, D, v[i]);
+  for (int i = 0; i < NCH; ++i) Elem<T>::template fetch8<FULL>(p, (tr + i * NT) * 8, D, w[i]);
+}
+template <int T, int NCH>
+DEVINL void open_row(const typename Elem<T>::raw8 (&w)[NCH], float (&v)[NCH][8]) {
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) Elem<T>::open8(w[i], v[i]);
 }
 
 // parameters are the tensors' own type or float32
 template <int T, int NCH, int NT>
 DEVINL void load_param(const void* p, int64_t off, int f32, int tr, int D, float (&v)[NCH][8], float dflt, float add) {
-  if (!p) {
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
+  for (int i = 0; i < NCH; ++i) {
+    if (!p) {
       for (int j = 0; j < 8; ++j) v[i][j] = dflt;
-    return;
+    } else {
+      if (f32) Elem<2>::load8((const float*)p + off, (tr + i * NT) * 8, D, v[i]);
+      else Elem<T>::load8((const typename Elem<T>::type*)p + off, (tr + i * NT) * 8, D, v[i]);
+      for (int j = 0; j < 8; ++j) v[i][j] += add;
+    }
   }
-  if (f32) load_row<2, NCH, NT>((const float*)p + off, tr, D, v);
-  else load_row<T, NCH, NT>((const typename Elem<T>::type*)p + off, tr, D, v);
-#pragma unroll
-  for (int i = 0; i < NCH; ++i)
-    for (int j = 0; j < 8; ++j) v[i][j] += add;
 }
 
-template <int T, int WPR, int NCH>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(LnArgs a) {
+// Both kernels walk rows with a stride of the grid and keep the next row's loads in flight while they reduce this one.  A row
+// group without a row left (the last round) repeats the sample's last row and drops what it computes: every wave meets every barrier.
+template <int T, int WPR, int NCH, bool FULL>
+__global__ __launch_bounds__(64 * WAVES, NCH == 1 ? 8 : 4) void ln_fwd_kernel(LnArgs a) {
   using E = typename Elem<T>::type;
-  constexpr int NT = 64 * WPR, RPB = 4 / WPR;
-  __shared__ float red[2][4];
+  constexpr int NT = 64 * WPR, RPB = WAVES / WPR;
+  __shared__ float2 red[2][WAVES];
   int turn = 0;
   const int tr = threadIdx.x % NT, sub = threadIdx.x / NT;
-  const int64_t b = blockIdx.y;
+  const int64_t b = blockIdx.y, step = (int64_t)gridDim.x * RPB;
+  const E* xb = (const E*)a.x + b * a.x_bs;
+  int64_t t0 = (int64_t)blockIdx.x * RPB;
+  typename Elem<T>::raw8 w[NCH];
+  fetch_row<T, NCH, NT, FULL>(xb + min(t0 + sub, a.T - 1) * a.x_rs, tr, a.D, w);
   float g[NCH][8], be[NCH][8];
   load_param<T, NCH, NT>(a.gamma, b * a.p_bs, a.p_f32, tr, a.D, g, 1.f, a.gamma ? a.offset : 0.f);
   load_param<T, NCH, NT>(a.beta, b * a.p_bs, a.p_f32, tr, a.D, be, 0.f, 0.f);
   const float inv = 1.0f / (float)a.D;
-  for (int64_t t0 = (int64_t)blockIdx.x * RPB; t0 < a.T; t0 += (int64_t)gridDim.x * RPB) {
+  for (; t0 < a.T; t0 += step) {
     const int64_t t = t0 + sub;
-    if (WPR == 1 && t >= a.T) break;                      // (WPR = 4: one row per block, t < T here; every wave meets the barriers)
     float v[NCH][8];
-    load_row<T, NCH, NT>((const E*)a.x + b * a.x_bs + t * a.x_rs, tr, a.D, v);
+    open_row<T, NCH>(w, v);
+    if (t0 + step < a.T) fetch_row<T, NCH, NT, FULL>(xb + min(t + step, a.T - 1) * a.x_rs, tr, a.D, w);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
       for (int j = 0; j < 8; ++j) s += v[i][j];           // elements behind the row's end are zeros
-    const float mu = row_sum<WPR>(s, red, turn) * inv;
+    const float mu = row_sum2<WPR>(s, 0.f, red, turn).x * inv;
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
@@ -93,32 +117,46 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnArgs a) {
         const float d = v[i][j] - mu;
         q += (tr + i * NT) * 8 + j < a.D ? d * d : 0.f;
       }
-    const float r = 1.0f / sqrtf(row_sum<WPR>(q, red, turn) * inv + a.eps);
-    const int64_t row = b * a.T + t;
-    E* y = (E*)a.y + row * a.D;
+    const float r = 1.0f / sqrtf(row_sum2<WPR>(q, 0.f, red, turn).x * inv + a.eps);
+    if (t < a.T) {
+      const int64_t row = b * a.T + t;
+      E* y = (E*)a.y + row * a.D;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      float o[8];
-      for (int j = 0; j < 8; ++j) o[j] = (v[i][j] - mu) * r * g[i][j] + be[i][j];
-      Elem<T>::store8(y, (tr + i * NT) * 8, a.D, o);
-    }
-    if (tr == 0) {
-      a.mean[row] = mu;
-      a.rstd[row] = r;
+      for (int i = 0; i < NCH; ++i) {
+        float o[8];
+        for (int j = 0; j < 8; ++j) o[j] = (v[i][j] - mu) * r * g[i][j] + be[i][j];
+        Elem<T>::template store8<FULL>(y, (tr + i * NT) * 8, a.D, o);
+      }
+      if (tr == 0) {
+        a.mean[row] = mu;
+        a.rstd[row] = r;
+      }
     }
   }
 }
 
 // PG: also the parameter gradient: one partial row [2][D] per block, or the gradient itself (a.direct).
-template <int T, int WPR, int NCH, bool PG>
-__global__ __launch_bounds__(256) void ln_bwd_kernel(LnArgs a) {
+template <int T, int WPR, int NCH, bool FULL, bool PG>
+__global__ __launch_bounds__(64 * WAVES, !PG ? (NCH == 1 ? 6 : 4) : NCH == 1 ? 4 : 2) void ln_bwd_kernel(LnArgs a) {
   using E = typename Elem<T>::type;
-  constexpr int NT = 64 * WPR, RPB = 4 / WPR;
-  __shared__ float red[2][4];
-  __shared__ float comb[PG && WPR == 1 ? 3 * 64 * NCH * 8 : 1];
+  constexpr int NT = 64 * WPR, RPB = WAVES / WPR;
+  __shared__ float2 red[2][WAVES];
+  __shared__ float comb[PG ? NCH * 8 * NT * RPB : 1];
   int turn = 0;
   const int tr = threadIdx.x % NT, sub = threadIdx.x / NT;
-  const int64_t b = blockIdx.y;
+  const int64_t b = blockIdx.y, step = (int64_t)gridDim.x * RPB;
+  const E *xb = (const E*)a.x + b * a.x_bs, *db_ = (const E*)a.dy + b * a.dy_bs;
+  int64_t t0 = (int64_t)blockIdx.x * RPB;
+  typename Elem<T>::raw8 wx[NCH], wd[NCH];
+  float mu, r;
+  auto fetch = [&](int64_t t) {
+    t = min(t, a.T - 1);
+    fetch_row<T, NCH, NT, FULL>(xb + t * a.x_rs, tr, a.D, wx);
+    fetch_row<T, NCH, NT, FULL>(db_ + t * a.dy_rs, tr, a.D, wd);
+    mu = a.mean[b * a.T + t];
+    r = a.rstd[b * a.T + t];
+  };
+  fetch(t0 + sub);
   float g[NCH][8], dg[PG ? NCH : 1][8], db[PG ? NCH : 1][8];
   load_param<T, NCH, NT>(a.gamma, b * a.p_bs, a.p_f32, tr, a.D, g, 1.f, a.gamma ? a.offset : 0.f);
   if constexpr (PG) {
@@ -127,74 +165,71 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnArgs a) {
       for (int j = 0; j < 8; ++j) dg[i][j] = db[i][j] = 0.f;
   }
   const float inv = 1.0f / (float)a.D;
-  for (int64_t t0 = (int64_t)blockIdx.x * RPB; t0 < a.T; t0 += (int64_t)gridDim.x * RPB) {
+  for (; t0 < a.T; t0 += step) {
     const int64_t t = t0 + sub;
-    if (WPR == 1 && t >= a.T) break;
-    const int64_t row = b * a.T + t;
-    float x[NCH][8], d[NCH][8];
-    load_row<T, NCH, NT>((const E*)a.x + b * a.x_bs + t * a.x_rs, tr, a.D, x);
-    load_row<T, NCH, NT>((const E*)a.dy + b * a.dy_bs + t * a.dy_rs, tr, a.D, d);
-    const float mu = a.mean[row], r = a.rstd[row];
+    const float on = t < a.T ? 1.f : 0.f;                 // a repeated row adds nothing to the parameter sums
+    typename Elem<T>::raw8 cx[NCH], cd[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      cx[i] = wx[i];
+      cd[i] = wd[i];
+    }
+    const float m = mu, rs = r;
+    if (t0 + step < a.T) fetch(t + step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
+    for (int i = 0; i < NCH; ++i) {
+      float x[8], d[8];
+      Elem<T>::open8(cx[i], x);
+      Elem<T>::open8(cd[i], d);
       for (int j = 0; j < 8; ++j) {
-        const float xh = (x[i][j] - mu) * r, dy = d[i][j], e = dy * g[i][j];   // dy is zero behind the row's end, so are all sums' terms
-        x[i][j] = xh;
-        d[i][j] = e;
+        const float xh = (x[j] - m) * rs, dy = d[j], e = dy * g[i][j];   // dy is zero behind the row's end, so are all sums' terms
         s1 += e;
         s2 += e * xh;
         if constexpr (PG) {
-          dg[i][j] += dy * xh;
-          db[i][j] += dy;
+          const float dyo = dy * on;
+          dg[i][j] += dyo * xh;
+          db[i][j] += dyo;
         }
       }
-    s1 = row_sum<WPR>(s1, red, turn) * inv;
-    s2 = row_sum<WPR>(s2, red, turn) * inv;
-    E* dx = (E*)a.y + row * a.D;
+      if constexpr (T < 2) asm volatile("" : "+v"(cx[i]), "+v"(cd[i]));  // unpack again below: half the registers across the reduction
+    }
+    const float2 s = row_sum2<WPR>(s1, s2, red, turn);
+    if (t < a.T) {
+      E* dx = (E*)a.y + (b * a.T + t) * a.D;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      float o[8];
-      for (int j = 0; j < 8; ++j) o[j] = r * (d[i][j] - s1 - x[i][j] * s2);
-      Elem<T>::store8(dx, (tr + i * NT) * 8, a.D, o);
+      for (int i = 0; i < NCH; ++i) {
+        float x[8], d[8], o[8];
+        Elem<T>::open8(cx[i], x);
+        Elem<T>::open8(cd[i], d);
+        for (int j = 0; j < 8; ++j) o[j] = rs * (d[j] * g[i][j] - s.x * inv - (x[j] - m) * rs * (s.y * inv));
+        Elem<T>::template store8<FULL>(dx, (tr + i * NT) * 8, a.D, o);
+      }
     }
   }
-  if constexpr (PG) {
-    if constexpr (WPR == 1) {                             // the four waves hold the same columns: add them in wave order
+  if constexpr (PG) {                                     // the row groups hold the same columns: add them in group order
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        auto& v = which ? db : dg;
-        __syncthreads();
-        if (sub > 0)
-          for (int i = 0; i < NCH; ++i)
-            for (int j = 0; j < 8; ++j) comb[((sub - 1) * NCH * 8 + i * 8 + j) * 64 + tr] = v[i][j];
-        __syncthreads();
-        if (sub == 0)
-          for (int w = 0; w < 3; ++w)
-            for (int i = 0; i < NCH; ++i)
-              for (int j = 0; j < 8; ++j) v[i][j] += comb[(w * NCH * 8 + i * 8 + j) * 64 + tr];
-      }
-      if (sub) return;
-    }
-    if (a.direct) {
-      const int64_t off = b * a.D;
+    for (int which = 0; which < 2; ++which) {
+      auto& v = which ? db : dg;
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        const int c = (tr + i * NT) * 8;
-        if (a.p_f32) {
-          Elem<2>::store8((float*)a.dgamma + off, c, a.D, dg[i]);
-          Elem<2>::store8((float*)a.dbeta + off, c, a.D, db[i]);
-        } else {
-          Elem<T>::store8((E*)a.dgamma + off, c, a.D, dg[i]);
-          Elem<T>::store8((E*)a.dbeta + off, c, a.D, db[i]);
+      for (int i = 0; i < NCH; ++i)
+        for (int j = 0; j < 8; ++j) comb[((sub * NCH + i) * 8 + j) * NT + tr] = v[i][j];
+      __syncthreads();
+      if (sub == which % RPB) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          float o[8];
+          for (int j = 0; j < 8; ++j) {
+            o[j] = 0.f;
+            for (int k = 0; k < RPB; ++k) o[j] += comb[((k * NCH + i) * 8 + j) * NT + tr];
+          }
+          const int c = (tr + i * NT) * 8;
+          void* out = which ? a.dbeta : a.dgamma;
+          if (!a.direct) Elem<2>::store8(a.part + ((b * gridDim.x + blockIdx.x) * 2 + which) * (int64_t)a.D, c, a.D, o);
+          else if (a.p_f32) Elem<2>::store8((float*)out + b * a.D, c, a.D, o);
+          else Elem<T>::store8((E*)out + b * a.D, c, a.D, o);
         }
-      }
-    } else {
-      float* part = a.part + ((b * gridDim.x + blockIdx.x) * 2) * (int64_t)a.D;
-#pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        Elem<2>::store8(part, (tr + i * NT) * 8, a.D, dg[i]);
-        Elem<2>::store8(part + a.D, (tr + i * NT) * 8, a.D, db[i]);
       }
     }
   }
@@ -204,7 +239,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnArgs a) {
 template <int T, bool BWD>
 __global__ __launch_bounds__(256) void ln_wide_kernel(LnArgs a) {
   using E = typename Elem<T>::type;
-  __shared__ float red[2][4];
+  __shared__ float2 red[2][WAVES];
   int turn = 0;
   const int64_t b = blockIdx.y;
   const float inv = 1.0f / (float)a.D, off = a.gamma ? a.offset : 0.f;
@@ -232,20 +267,21 @@ __global__ __launch_bounds__(256) void ln_wide_kernel(LnArgs a) {
           s2 += e * (v[j] - mu) * r;
         }
       }
-      s1 = row_sum<4>(s1, red, turn) * inv;
-      s2 = row_sum<4>(s2, red, turn) * inv;
+      const float2 t2 = row_sum2<4>(s1, s2, red, turn);
+      s1 = t2.x * inv;
+      s2 = t2.y * inv;
     } else {
       float s = 0.f, q = 0.f;
       for (int c = threadIdx.x * 8; c < a.D; c += 2048) {
         Elem<T>::load8(x, c, a.D, v);
         for (int j = 0; j < 8; ++j) s += v[j];
       }
-      mu = row_sum<4>(s, red, turn) * inv;
+      mu = row_sum2<4>(s, 0.f, red, turn).x * inv;
       for (int c = threadIdx.x * 8; c < a.D; c += 2048) {
         Elem<T>::load8(x, c, a.D, v);
         for (int j = 0; j < 8; ++j) q += c + j < a.D ? (v[j] - mu) * (v[j] - mu) : 0.f;
       }
-      r = 1.0f / sqrtf(row_sum<4>(q, red, turn) * inv + a.eps);
+      r = 1.0f / sqrtf(row_sum2<4>(q, 0.f, red, turn).x * inv + a.eps);
       if (threadIdx.x == 0) {
         a.mean[row] = mu;
         a.rstd[row] = r;
@@ -288,66 +324,90 @@ __global__ __launch_bounds__(256) void ln_wide_param_kernel(LnArgs a) {
   Elem<2>::store8(part + a.D, c, a.D, db);
 }
 
-// Waves per row and chunks per lane.  Many rows: a wave per row while the row fits 4 chunks a lane (no barrier in the loop);
-// few rows: four waves share one, a quarter of the serial work each.
+// Waves per row and chunks per lane.  Few rows, float32, a parameter gradient or a width that cuts a chunk: as many waves as give
+// a lane one chunk - short serial work, and registers stay free for the loads in flight.  Else two or three chunks a lane, which
+// leaves fewer idle lanes and fewer barriers.  Measured (us, several chunks / one): 16384 x 1280 f16 forward 20.2 / 23.4, dx alone
+// 24.1 / 24.8, with parameter gradient 45.4 / 42.2; 4 x 4096 x 2560 bf16 36.4 / 40.6, 41.8 / 43.1, 59.0 / 52.9; 16384 x 1280
+// float32 32.3 / 30.1, 62.9 / 41.7, 62.8 / 55.6.
 struct Shape { int wpr, nch; };
-Shape pick(int64_t rows, int D) {
+Shape pick(int64_t rows, int D, bool f32, bool pg) {
   const int c = (D + 7) / 8;
+  const bool several = rows >= 2048 && !f32 && !pg && D % 8 == 0;
   if (c <= 64) return {1, 1};
-  if (c <= 256 && rows < 2048) return {4, 1};
-  if (c <= 256) return {1, (c + 63) / 64};
-  if (c <= 512) return {4, 2};
-  if (c <= 1024) return {4, 4};
+  if (several && c <= 192) return {1, (c + 63) / 64};
+  if (c <= 128) return {2, 1};
+  if (c <= 256) return {4, 1};
+  if (several && c <= 384) return {4, 2};
+  if (c <= 512) return {8, 1};
+  if (c <= 1024) return {8, 2};
   return {0, 0};
 }
-// partial rows per sample: about two blocks a CU in all, and no more than there are row groups
+int64_t row_groups(int64_t T, Shape s) {
+  const int64_t rpb = s.wpr == 0 ? 1 : WAVES / s.wpr;
+  return (T + rpb - 1) / rpb;
+}
+// blocks per sample: `most` in all, every block the same number of rounds (but the last)
+int64_t even_blocks(int64_t B, int64_t groups, int64_t most) {
+  const int64_t n = most / (B < most ? B : most), rounds = (groups + n - 1) / n;
+  return (groups + rounds - 1) / rounds;
+}
+// partial rows per sample.  Two blocks a CU in all; at least four rounds a block, since every partial row is read again.
 int64_t partials(int64_t B, int64_t T, int D, Shape s) {
-  const int64_t rpb = s.wpr == 1 ? 4 : 1, groups = (T + rpb - 1) / rpb;
+  const int64_t groups = row_groups(T, s);
   if (groups <= 4 && s.wpr) return 1;                     // a handful of rows: one block, no second launch
-  int64_t n = 512 / (B < 512 ? B : 512);
-  if (!s.wpr) n = 64;
-  return n < 1 ? 1 : n < groups ? n : groups;
+  if (!s.wpr) return groups < 64 ? groups : 64;
+  const int64_t n = even_blocks(B, groups, 512);
+  return n > (groups + 3) / 4 ? (groups + 3) / 4 : n;
 }
 
 #define LN_DISPATCH(KERNEL, ...)                                              \
   if (s.wpr == 1 && s.nch == 1) KERNEL(1, 1, __VA_ARGS__);                    \
   else if (s.wpr == 1 && s.nch == 2) KERNEL(1, 2, __VA_ARGS__);               \
-  else if (s.wpr == 1 && s.nch == 3) KERNEL(1, 3, __VA_ARGS__);               \
-  else if (s.wpr == 1) KERNEL(1, 4, __VA_ARGS__);                             \
-  else if (s.nch == 1) KERNEL(4, 1, __VA_ARGS__);                             \
-  else if (s.nch == 2) KERNEL(4, 2, __VA_ARGS__);                             \
-  else KERNEL(4, 4, __VA_ARGS__)
+  else if (s.wpr == 1) KERNEL(1, 3, __VA_ARGS__);                             \
+  else if (s.wpr == 2) KERNEL(2, 1, __VA_ARGS__);                             \
+  else if (s.wpr == 4 && s.nch == 1) KERNEL(4, 1, __VA_ARGS__);               \
+  else if (s.wpr == 4) KERNEL(4, 2, __VA_ARGS__);                             \
+  else if (s.nch == 1) KERNEL(8, 1, __VA_ARGS__);                             \
+  else KERNEL(8, 2, __VA_ARGS__)
 
 template <int T>
 void launch_fwd(const LnArgs& a, int64_t B, hipStream_t st) {
-  const Shape s = pick(B * a.T, a.D);
-  const int64_t rpb = s.wpr == 1 ? 4 : 1, groups = (a.T + rpb - 1) / rpb, cap = B < 2048 ? 4096 / B : 2;
-  const dim3 grid((unsigned)(groups < cap ? groups : cap), (unsigned)B);
+  const Shape s = pick(B * a.T, a.D, T == 2, false);
+  const dim3 grid((unsigned)even_blocks(B, row_groups(a.T, s), 1024), (unsigned)B);
   if (!s.wpr) {
     hipLaunchKernelGGL((ln_wide_kernel<T, false>), grid, dim3(256), 0, st, a);
     return;
   }
-#define LN_F(W, N, X) hipLaunchKernelGGL((ln_fwd_kernel<T, W, N>), grid, dim3(256), 0, st, a)
-  LN_DISPATCH(LN_F, 0);
+#define LN_F(W, N, FULL) hipLaunchKernelGGL((ln_fwd_kernel<T, W, N, FULL>), grid, dim3(64 * WAVES), 0, st, a)
+  if (a.D % 8 == 0) {
+    LN_DISPATCH(LN_F, true);
+  } else {
+    LN_DISPATCH(LN_F, false);
+  }
 #undef LN_F
 }
 
 template <int T>
 void launch_bwd(LnArgs a, int64_t B, hipStream_t st) {
-  const Shape s = pick(B * a.T, a.D);
   const bool pg = a.dgamma != nullptr, shared = pg && a.p_bs == 0;
-  const int64_t rpb = s.wpr == 1 ? 4 : 1, groups = (a.T + rpb - 1) / rpb, cap = B < 2048 ? 4096 / B : 2;
-  const int64_t np = partials(B, a.T, a.D, s), nx = pg && s.wpr ? np : groups < cap ? groups : cap;
+  const Shape s = pick(B * a.T, a.D, T == 2, pg);
+  const int64_t np = partials(B, a.T, a.D, s), nx = pg && s.wpr ? np : even_blocks(B, row_groups(a.T, s), 1024);
   const dim3 grid((unsigned)nx, (unsigned)B);
   a.direct = s.wpr && np == 1 && (B == 1 || !shared);
   if (!s.wpr) {
     hipLaunchKernelGGL((ln_wide_kernel<T, true>), grid, dim3(256), 0, st, a);
     if (pg) hipLaunchKernelGGL((ln_wide_param_kernel<T>), dim3((a.D + 2047) / 2048, (unsigned)np, (unsigned)B), dim3(256), 0, st, a);
   } else if (pg) {
-#define LN_B(W, N, PG) hipLaunchKernelGGL((ln_bwd_kernel<T, W, N, PG>), grid, dim3(256), 0, st, a)
-    LN_DISPATCH(LN_B, true);
+#define LN_B(W, N, FULL, PG) hipLaunchKernelGGL((ln_bwd_kernel<T, W, N, FULL, PG>), grid, dim3(64 * WAVES), 0, st, a)
+    if (a.D % 8 == 0) {
+      LN_DISPATCH(LN_B, true, true);
+    } else {
+      LN_DISPATCH(LN_B, false, true);
+    }
+  } else if (a.D % 8 == 0) {
+    LN_DISPATCH(LN_B, true, false);
   } else {
-    LN_DISPATCH(LN_B, false);
+    LN_DISPATCH(LN_B, false, false);
 #undef LN_B
   }
   if (pg && !a.direct) {
@@ -365,7 +425,7 @@ bool bad_shape(int64_t B, int64_t T, int64_t D, int dtype) {
 
 extern "C" int64_t fluxhip_layernorm_grad_ws(int64_t B, int64_t T, int D) {
   if (bad_shape(B, T, D, 0)) return FLUXHIP_EINVAL;
-  return B * partials(B, T, D, pick(B * T, D)) * 2 * D * 4;
+  return B * partials(B, T, D, pick(B * T, D, false, true)) * 2 * D * 4;
 }
 
 extern "C" int fluxhip_layernorm_stats(const void* x, int64_t x_bs, int64_t x_rs, const void* gamma, const void* beta, int64_t p_bs,

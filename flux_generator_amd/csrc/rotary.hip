@@ -6,8 +6,8 @@
 //
 // The angle is formed in 64 bits - at position 10^6 a float32 product is off by 0.06 rad - and reduced to a fraction of a turn
 // there; cos / sin of the fraction are float32.  A block takes TB consecutive tokens: one thread per (token, pair) computes the
-// pair's cos and sin ONCE into LDS, then all threads walk the tokens' heads in vectors of V elements; a thread keeps its column
-// and moves over heads, so a token's q and k heads (and the values between them in a fused projection) need no index division.
+// pair's cos and sin ONCE into LDS, then all threads walk the tokens' q and k heads in vectors of V elements; a thread keeps its
+// columns and moves over (token, head) items.
 #include "../../include/fluxhip.h"
 #include "common.h"
 #include "elem.h"
@@ -26,102 +26,118 @@ struct RopeArgs {
   int64_t pb, pt, ntok;                // element strides of the positions; B * T
   int pos64, n_axes, ax1, ax2, ax3;    // first pair of axis 1, 2, 3
   int T, H, K, hd, rot, tb, slots, lanes;
+  uint32_t magic;                      // ceil(2^32 / heads): i / heads = umulhi(i, magic) for i heads < 2^32
   float scale;
 };
 
+// V elements as they lie in memory
 template <int T, int V>
-DEVINL void vload(const typename Elem<T>::type* p, float (&v)[V]) {
+struct Vec {
   typename Elem<T>::type w[V];
-  __builtin_memcpy(w, p, sizeof(w));
-#pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = Elem<T>::get(&w[j]);
-}
-template <int T, int V>
-DEVINL void vstore(typename Elem<T>::type* p, const float (&v)[V]) {
-  typename Elem<T>::type w[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) Elem<T>::put(&w[j], v[j]);
-  __builtin_memcpy(p, w, sizeof(w));
-}
+  DEVINL void load(const typename Elem<T>::type* p) { __builtin_memcpy(w, p, sizeof(w)); }
+  DEVINL void store(typename Elem<T>::type* p) const { __builtin_memcpy(p, w, sizeof(w)); }
+  DEVINL float get(int j) const { return Elem<T>::get(&w[j]); }
+  DEVINL void put(int j, float v) { Elem<T>::put(&w[j], v); }
+};
 
-// V: elements per vector (interleaved: V / 2 pairs; half: V pairs, two vectors), dividing the rotated columns
+// V: elements per vector (interleaved: V / 2 pairs; half: V pairs, two vectors), dividing the rotated columns.  A thread takes
+// UNROLL (token, head) items at a time, all loads before the first use; the first batch's loads go out before the block works on
+// its angles.
 template <int T, int V, bool INTER, bool INV>
 __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
   using E = typename Elem<T>::type;
+  constexpr int UNROLL = V * sizeof(E) == 16 && INTER ? 4 : 2;
   extern __shared__ float2 cs[];       // [tb][rot / 2]
   const int np = a.rot >> 1;
-  const int64_t tok0 = (int64_t)blockIdx.x * a.tb;
-  const int ntb = (int)(a.ntok - tok0 < a.tb ? a.ntok - tok0 : a.tb);
-  const int64_t b0 = tok0 / a.T;
-  const int t0 = (int)(tok0 - b0 * a.T);
+  const int64_t tok0 = (int64_t)blockIdx.x * a.tb, b0 = tok0 / a.T;
+  const int ntb = (int)(a.ntok - tok0 < a.tb ? a.ntok - tok0 : a.tb), t0 = (int)(tok0 - b0 * a.T);
+
+  const int heads = a.H + a.K, per = 256 / a.lanes;       // `lanes` threads cover a head's slots, `per` heads side by side
+  const int row = threadIdx.x / a.lanes, lane = threadIdx.x - row * a.lanes;
+  const int rot_slots = INTER ? a.rot / V : np / V, step = per * gridDim.y, items = row < per ? ntb * heads : 0;
+  const int first = row + blockIdx.y * per;
+
+  const E* x[UNROLL];
+  E* y[UNROLL];
+  int tk[UNROLL];
+  Vec<T, V> p[UNROLL], q[INTER ? 1 : UNROLL];
+  auto fetch = [&](int it, int slot) {                    // items it, it + step, ..: an item behind the end repeats the last one
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = min(it + u * step, items - 1);
+      tk[u] = (int)__umulhi((uint32_t)i, a.magic);        // i / heads
+      if (heads == 1) tk[u] = i;
+      const int h = i - tk[u] * heads;
+      uint32_t t = t0 + tk[u], bq = t / (uint32_t)a.T;
+      t -= bq * a.T;
+      const int64_t b = b0 + bq;
+      const bool isk = h >= a.H;
+      const RopeTensor& r = isk ? a.k : a.q;
+      const int64_t hh = isk ? h - a.H : h;
+      x[u] = (const E*)r.x + b * r.xb + t * r.xt + hh * r.xh;
+      y[u] = (E*)r.y + b * r.yb + t * r.yt + hh * r.yh;
+      if (slot < rot_slots) {
+        p[u].load(x[u] + slot * V);
+        if constexpr (!INTER) q[u].load(x[u] + np + slot * V);
+      }
+    }
+  };
+  if (first < items && lane < a.slots) fetch(first, lane);
+
   for (int i = threadIdx.x; i < ntb * np; i += 256) {
-    const int tk = i / np, j = i - tk * np;
-    int64_t b = b0;
-    int t = t0 + tk;
-    while (t >= a.T) { t -= a.T; ++b; }
+    const int k = i / np, j = i - k * np;
+    uint32_t t = t0 + k;
+    const uint32_t bq = t / (uint32_t)a.T;
+    t -= bq * a.T;
     const int ax = (j >= a.ax1) + (j >= a.ax2) + (j >= a.ax3);
-    const int64_t at = b * a.pb + t * a.pt + ax;
-    const double p = a.pos64 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
-    const double turns = p * a.freq[j] * 0.15915494309189533576888;
+    const int64_t at = (b0 + bq) * a.pb + t * a.pt + ax;
+    const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
+    const double turns = pos * a.freq[j] * 0.15915494309189533576888;
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     cs[i] = make_float2(c * a.scale, INV ? -s * a.scale : s * a.scale);
   }
   __syncthreads();
-  const int heads = a.H + a.K, per = 256 / a.lanes;       // `lanes` threads cover a head's slots, `per` heads side by side
-  const int lane = threadIdx.x % a.lanes;
-  if ((int)threadIdx.x >= per * a.lanes) return;
-  const int rot_slots = INTER ? a.rot / V : np / V;
+
   for (int slot = lane; slot < a.slots; slot += a.lanes) {
-    int64_t b = b0;
-    int tk = 0, t = t0, h = threadIdx.x / a.lanes + blockIdx.y * per;
-    const int step = per * gridDim.y;
-    while (true) {
-      while (h >= heads) {
-        h -= heads;
-        ++tk;
-        if (++t == a.T) { t = 0; ++b; }
-      }
-      if (tk >= ntb) break;
-      const bool isk = h >= a.H;
-      const RopeTensor& r = isk ? a.k : a.q;
-      const int64_t hh = isk ? h - a.H : h;
-      const E* x = (const E*)r.x + b * r.xb + t * r.xt + hh * r.xh;
-      E* y = (E*)r.y + b * r.yb + t * r.yt + hh * r.yh;
-      const float2* w = cs + tk * np;
-      if (slot >= rot_slots) {                            // behind the rotated part
-        const int c = a.rot + (slot - rot_slots) * V;
-        if (c + V <= a.hd) {
-          float v[V];
-          vload<T, V>(x + c, v);
-          vstore<T, V>(y + c, v);
+    for (int it = first; it < items; it += step * UNROLL) {
+      if (it != first || slot != lane) fetch(it, slot);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (it + u * step >= items) break;
+        const float2* w = cs + tk[u] * np;
+        if (slot >= rot_slots) {                          // behind the rotated part
+          const int c = a.rot + (slot - rot_slots) * V;
+          if (c + V <= a.hd) {
+            Vec<T, V> v;
+            v.load(x[u] + c);
+            v.store(y[u] + c);
+          } else {
+            for (int e = c; e < a.hd; ++e) y[u][e] = x[u][e];
+          }
+        } else if constexpr (INTER) {
+          Vec<T, V> o;
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            const float2 c = w[slot * (V / 2) + j];
+            const float m = p[u].get(2 * j), n = p[u].get(2 * j + 1);
+            o.put(2 * j, m * c.x - n * c.y);
+            o.put(2 * j + 1, m * c.y + n * c.x);
+          }
+          o.store(y[u] + slot * V);
         } else {
-          for (int e = c; e < a.hd; ++e) y[e] = x[e];
-        }
-      } else if constexpr (INTER) {
-        float v[V], o[V];
-        vload<T, V>(x + slot * V, v);
+          Vec<T, V> o1, o2;
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) {
-          const float2 u = w[slot * (V / 2) + j];
-          o[2 * j] = v[2 * j] * u.x - v[2 * j + 1] * u.y;
-          o[2 * j + 1] = v[2 * j] * u.y + v[2 * j + 1] * u.x;
+          for (int j = 0; j < V; ++j) {
+            const float2 c = w[slot * V + j];
+            const float m = p[u].get(j), n = q[u].get(j);
+            o1.put(j, m * c.x - n * c.y);
+            o2.put(j, m * c.y + n * c.x);
+          }
+          o1.store(y[u] + slot * V);
+          o2.store(y[u] + np + slot * V);
         }
-        vstore<T, V>(y + slot * V, o);
-      } else {
-        float p[V], q[V], o1[V], o2[V];
-        vload<T, V>(x + slot * V, p);
-        vload<T, V>(x + np + slot * V, q);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float2 u = w[slot * V + j];
-          o1[j] = p[j] * u.x - q[j] * u.y;
-          o2[j] = p[j] * u.y + q[j] * u.x;
-        }
-        vstore<T, V>(y + slot * V, o1);
-        vstore<T, V>(y + np + slot * V, o2);
       }
-      h += step;
     }
   }
 }
@@ -155,7 +171,7 @@ extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   if (pairs != d->rot / 2) return FLUXHIP_EINVAL;
   const int64_t ntok = d->B * d->T;
   if (ntok == 0 || d->H + d->K == 0) return FLUXHIP_OK;
-  if (d->T > (1ll << 31) - 1 || !d->positions || !d->freqs || (d->H && (!d->q || !d->q_out)) || (d->K && (!d->k || !d->k_out))) return FLUXHIP_EINVAL;
+  if (d->T > (1 << 30) || d->H > 4096 || d->K > 4096 || !d->positions || !d->freqs || (d->H && (!d->q || !d->q_out)) || (d->K && (!d->k || !d->k_out))) return FLUXHIP_EINVAL;
   RopeArgs a{};
   a.q = {d->q, d->q_out, d->q_strides[0], d->q_strides[1], d->q_strides[2], d->qo_strides[0], d->qo_strides[1], d->qo_strides[2]};
   a.k = {d->k, d->k_out, d->k_strides[0], d->k_strides[1], d->k_strides[2], d->ko_strides[0], d->ko_strides[1], d->ko_strides[2]};
@@ -170,6 +186,7 @@ extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   a.slots = part / V + (tail + V - 1) / V;
   a.lanes = a.slots < 256 ? a.slots : 256;
   const int per = 256 / a.lanes, heads = d->H + d->K, np = d->rot / 2;
+  a.magic = (uint32_t)(((1ull << 32) + heads - 1) / heads);
   // tokens per block: one sincos per thread (256 / pairs tokens), fewer while the launch would leave CUs idle; with few tokens
   // the heads are spread over blocks instead
   int tb = 256 / np > 1 ? 256 / np : 1;

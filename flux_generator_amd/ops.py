@@ -953,18 +953,29 @@ def attention_x3(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, H: int, Tk:
 _DT = {BF16: 0, F16: 1, F32: 2}
 
 
-def _on_device(*named) -> None:
-    """Every given (tensor, name) pair lives on the current device, whose stream the launch goes to."""
-    dev = None
+def _launch_stream(*named) -> int:
+    """The current stream (raw handle) of the current device, on which every given (tensor, name) pair must live."""
+    dev = -2
     for t, name in named:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise FluxHipError("libfluxhip ops need device tensors (no CPU fallback exists)")
-        if dev is None:
-            dev = torch.cuda.current_device()
-        if t.get_device() != dev:
-            raise FluxHipError(f"{name} is on {t.device}, the current device is cuda:{dev} (one process drives one GPU)")
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
+                raise FluxHipError("libfluxhip ops need device tensors (no CPU fallback exists)")
+            if dev >= 0 or d != torch.cuda.current_device():
+                raise FluxHipError(f"{name} is on cuda:{d}, the current device is cuda:{torch.cuda.current_device()} (one process drives one GPU)")
+            dev = d
+    return torch._C._cuda_getCurrentRawStream(dev)       # (torch.cuda.current_stream() builds an object: 2.7 us a call)
+
+
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor like t (half the cost of torch.empty with its keywords)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _samples(t: torch.Tensor, name: str, per_sample: bool):
@@ -1035,14 +1046,13 @@ def layernorm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optio
     [x.shape[:-1]].  x [..., D] bf16 / f16 / f32, any D, rows at one stride inside a sample (slices of packed buffers work).
     gamma, beta: [D], or one vector per sample [x.shape[0], D] (adaLN); unit_offset multiplies by 1 + gamma."""
     per, pf, (B, T, bs, rs), _ = _norm_args(x, gamma, beta)
-    _on_device((x, "x"), (gamma, "gamma"), (beta, "beta"))
+    st = _launch_stream((x, "x"), (gamma, "gamma"), (beta, "beta"))
     D = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=F32, device=x.device)
-    rstd = torch.empty(x.shape[:-1], dtype=F32, device=x.device)
-    _check(_lib.load().fluxhip_layernorm_stats(x.data_ptr(), bs, rs, _p(gamma), _p(beta), D if per else 0, int(pf),
+    y, mean = _new(x), x.new_empty(x.shape[:-1], dtype=F32)
+    rstd = torch.empty_like(mean)
+    _check(_lib.load().fluxhip_layernorm_stats(x.data_ptr(), bs, rs, _ptr(gamma), _ptr(beta), D if per else 0, int(pf),
                                                1.0 if unit_offset else 0.0, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), B, T, D,
-                                               eps, _DT[x.dtype], _stream()), "fluxhip_layernorm_stats")
+                                               eps, _DT[x.dtype], st), "fluxhip_layernorm_stats")
     return y, mean, rstd
 
 
@@ -1054,9 +1064,9 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rs
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         if t.dtype != F32 or not t.is_contiguous() or t.shape != x.shape[:-1]:
             raise FluxHipError(f"{name} must be the contiguous float32 [{', '.join(map(str, x.shape[:-1]))}] of layernorm")
-    _on_device((x, "x"), (dy, "dy"), (gamma, "gamma"), (mean, "mean"), (rstd, "rstd"))
+    st = _launch_stream((x, "x"), (dy, "dy"), (gamma, "gamma"), (mean, "mean"), (rstd, "rstd"))
     lib, D = _lib.load(), x.shape[-1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _new(x)
     dg = db = ws = None
     n = 0
     if gamma is not None and param_grads:
@@ -1064,10 +1074,10 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rs
             return dx, torch.zeros_like(gamma), torch.zeros_like(gamma)
         dg, db = torch.empty_like(gamma), torch.empty_like(gamma)
         n = lib.fluxhip_layernorm_grad_ws(B, T, D)
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-    _check(lib.fluxhip_layernorm_grad(dy.data_ptr(), dbs, drs, x.data_ptr(), bs, rs, mean.data_ptr(), rstd.data_ptr(), _p(gamma),
-                                      D if per else 0, int(pf), 1.0 if unit_offset else 0.0, dx.data_ptr(), _p(dg), _p(db), B, T, D,
-                                      _DT[x.dtype], _p(ws), n, _stream()), "fluxhip_layernorm_grad")
+        ws = x.new_empty(n, dtype=torch.uint8) if n else None
+    _check(lib.fluxhip_layernorm_grad(dy.data_ptr(), dbs, drs, x.data_ptr(), bs, rs, mean.data_ptr(), rstd.data_ptr(), _ptr(gamma),
+                                      D if per else 0, int(pf), 1.0 if unit_offset else 0.0, dx.data_ptr(), _ptr(dg), _ptr(db), B, T, D,
+                                      _DT[x.dtype], _ptr(ws), n, st), "fluxhip_layernorm_grad")
     return dx, dg, db
 
 
@@ -1125,39 +1135,33 @@ def _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, inverse, out):
     ps = positions.stride()
     pb = ps[0] if positions.dim() == len(lead) + 1 else 0
     pt = ps[-1] if na == 1 else ps[-2]
-    outs = [None, None] if out is None else ([out, None] if isinstance(out, torch.Tensor) else list(out))
+    outs = (None, None) if out is None else ((out, None) if isinstance(out, torch.Tensor) else tuple(out))
     if len(outs) != 2 or (k is None and outs[1] is not None) or (out is not None and k is not None and outs[1] is None):
         raise FluxHipError("out must give one tensor for each of q and k")
-    d = RotaryDesc()
-    got = []
-    for t, o, name in ((q, outs[0], "q"), (k, outs[1], "k")):
-        if t is None:
-            continue
-        if t.stride(-1) != 1 and hd != 1:
+
+    def place(t, o, name):
+        s = t.stride()
+        if s[3] != 1 and hd != 1:
             raise FluxHipError(f"{name} must have a contiguous last dimension")
         if o is None:
-            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        elif o.shape != t.shape or o.dtype != t.dtype or o.stride(-1) != 1:
+            o = _new(t)
+            return o, s[:3], o.stride()[:3]
+        if o.shape != t.shape or o.dtype != t.dtype or (o.stride(3) != 1 and hd != 1):
             raise FluxHipError(f"out must have {name}'s shape and type and a contiguous last dimension")
-        got.append(o)
-        s, so = t.stride(), o.stride()
-        if any(so[i] == 0 and t.shape[i] > 1 for i in range(3)):
+        if any(o.stride(i) == 0 and t.shape[i] > 1 for i in range(3)):
             raise FluxHipError("out must not be a broadcast view")
-        if name == "q":
-            d.q_strides[:], d.qo_strides[:] = s[:3], so[:3]
-        else:
-            d.k_strides[:], d.ko_strides[:] = s[:3], so[:3]
-    _on_device((q, "q"), (k, "k"), (positions, "positions"), (freqs, "freqs"), *((o, "out") for o in got))
-    d.q, d.q_out = q.data_ptr(), got[0].data_ptr()
+        return o, s[:3], o.stride()[:3]
+
+    qo, qs, qos = place(q, outs[0], "q")
+    K, ks, kos, ko, kp, kop = 0, (0, 0, 0), (0, 0, 0), None, None, None
     if k is not None:
-        d.k, d.k_out, d.K = k.data_ptr(), got[1].data_ptr(), k.shape[2]
-    d.positions, d.freqs, d.pos64 = positions.data_ptr(), freqs.data_ptr(), positions.dtype == torch.int64
-    d.pos_strides[:] = (pb, pt)
-    d.B, d.T, d.H, d.hd, d.rot, d.n_axes = B, T, H, hd, rot, na
-    d.axis_pairs[:na] = [w // 2 for w in dims]
-    d.interleaved, d.inverse, d.dtype, d.scale = interleaved, inverse, _DT[q.dtype], scale
-    _check(_lib.load().fluxhip_rotary(ctypes.byref(d), _stream()), "fluxhip_rotary")
-    return got[0] if k is None else (got[0], got[1])
+        ko, ks, kos = place(k, outs[1], "k")
+        K, kp, kop = k.shape[2], k.data_ptr(), ko.data_ptr()
+    st = _launch_stream((q, "q"), (k, "k"), (positions, "positions"), (freqs, "freqs"), (qo, "out"), (ko, "out"))
+    d = RotaryDesc(q.data_ptr(), kp, qo.data_ptr(), kop, qs, ks, qos, kos, positions.data_ptr(), freqs.data_ptr(), (pb, pt), B, T, H, K, hd, rot,
+                   interleaved, inverse, positions.dtype == torch.int64, na, tuple([w // 2 for w in dims]), _DT[q.dtype], scale)
+    _check(_lib.load().fluxhip_rotary(d, st), "fluxhip_rotary")
+    return qo if k is None else (qo, ko)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, axes_dim=None,
@@ -1220,22 +1224,17 @@ def gated_ff(x: torch.Tensor, w_value: torch.Tensor, w_gate: torch.Tensor, w_out
     for t, name, n in ((b_value, "b_value", F), (b_gate, "b_gate", F), (b_out, "b_out", D)):
         if t is not None and (tuple(t.shape) != (n,) or t.dtype != x.dtype or not t.is_contiguous()):
             raise FluxHipError(f"{name} must be a contiguous [{n}] tensor of {x.dtype}")
-    _on_device((x, "x"), (w_value, "w_value"), (w_gate, "w_gate"), (w_out, "w_out"), (b_value, "b_value"), (b_gate, "b_gate"), (b_out, "b_out"))
-    lib, lead = _lib.load(), x.shape[:-1]
-    y = torch.empty(*lead, D, dtype=x.dtype, device=x.device)
-    hidden = torch.empty(*lead, F, dtype=x.dtype, device=x.device)
+    st = _launch_stream((x, "x"), (w_value, "w_value"), (w_gate, "w_gate"), (w_out, "w_out"), (b_value, "b_value"), (b_gate, "b_gate"),
+                        (b_out, "b_out"))
+    lib = _lib.load()
+    y, hidden = _new(x), x.new_empty((*x.shape[:-1], F))
     saved = (torch.empty_like(hidden), torch.empty_like(hidden), hidden) if save else None
-    d = GatedFfDesc()
     n = lib.fluxhip_gated_ff_ws(M, D, F)
-    if n > 0:
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        d.ws, d.ws_bytes = ws.data_ptr(), n
-    d.x, d.w_value, d.w_gate, d.w_out, d.hidden, d.y = (t.data_ptr() for t in (x, w_value, w_gate, w_out, hidden, y))
-    d.b_value, d.b_gate, d.b_out = _p(b_value), _p(b_gate), _p(b_out)
-    if save:
-        d.value, d.gate = saved[0].data_ptr(), saved[1].data_ptr()
-    d.M, d.ldx, d.D, d.F, d.act, d.dtype = M, ldx, D, F, act, _DT[x.dtype]
-    _check(lib.fluxhip_gated_ff(ctypes.byref(d), _stream()), "fluxhip_gated_ff")
+    ws = x.new_empty(n, dtype=torch.uint8) if n > 0 else None
+    d = GatedFfDesc(x.data_ptr(), w_value.data_ptr(), w_gate.data_ptr(), w_out.data_ptr(), _ptr(b_value), _ptr(b_gate), _ptr(b_out),
+                    saved[0].data_ptr() if save else None, saved[1].data_ptr() if save else None, hidden.data_ptr(), y.data_ptr(), M, ldx, D, F,
+                    act, _DT[x.dtype], _ptr(ws), n)
+    _check(lib.fluxhip_gated_ff(d, st), "fluxhip_gated_ff")
     return (y, saved) if save else y
 
 
@@ -1252,26 +1251,22 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, saved, w_value: torch.T
     for t, name in ((value, "value"), (gate, "gate"), (hidden, "hidden")):
         if t.shape != (*x.shape[:-1], F) or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16:
             raise FluxHipError(f"{name} must be the contiguous [..., {F}] tensor gated_ff saved")
-    _on_device((x, "x"), (dy, "dy"), (value, "value"), (gate, "gate"), (hidden, "hidden"), (w_value, "w_value"), (w_gate, "w_gate"),
-               (w_out, "w_out"))
+    st = _launch_stream((x, "x"), (dy, "dy"), (value, "value"), (gate, "gate"), (hidden, "hidden"), (w_value, "w_value"), (w_gate, "w_gate"),
+                        (w_out, "w_out"))
     lib = _lib.load()
-    new = lambda t: torch.empty(t.shape, dtype=x.dtype, device=x.device)
-    dx = new(x) if input_grad else None
-    dw = [new(w) for w in (w_value, w_gate, w_out)] if weight_grads else [None] * 3
-    db = [torch.empty(n, dtype=x.dtype, device=x.device) for n in (F, F, D)] if bias_grads else [None] * 3
+    dx = _new(x) if input_grad else None
+    dw = [_new(w) for w in (w_value, w_gate, w_out)] if weight_grads else [None] * 3
+    db = [x.new_empty(n) for n in (F, F, D)] if bias_grads else [None] * 3
     if M == 0:
         for t in dw + db:
             if t is not None:
                 t.zero_()
         return (dx, *dw, *db)
-    dvalue, dgate = new(value), new(value)
-    d = GatedFfGradDesc()
+    dvalue, dgate = _new(value), _new(value)
     n = lib.fluxhip_gated_ff_grad_ws(M, D, F)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-    d.ws, d.ws_bytes = ws.data_ptr(), n
-    d.dy, d.x, d.value, d.gate, d.hidden = (t.data_ptr() for t in (dy, x, value, gate, hidden))
-    d.w_value, d.w_gate, d.w_out, d.dvalue, d.dgate = (t.data_ptr() for t in (w_value, w_gate, w_out, dvalue, dgate))
-    d.dx, d.dw_value, d.dw_gate, d.dw_out, d.db_value, d.db_gate, d.db_out = (_p(t) for t in (dx, *dw, *db))
-    d.M, d.ldx, d.lddy, d.D, d.F, d.act, d.dtype = M, ldx, lddy, D, F, act, _DT[x.dtype]
-    _check(lib.fluxhip_gated_ff_grad(ctypes.byref(d), _stream()), "fluxhip_gated_ff_grad")
+    ws = x.new_empty(n, dtype=torch.uint8)
+    d = GatedFfGradDesc(dy.data_ptr(), x.data_ptr(), value.data_ptr(), gate.data_ptr(), hidden.data_ptr(), w_value.data_ptr(), w_gate.data_ptr(),
+                        w_out.data_ptr(), dvalue.data_ptr(), dgate.data_ptr(), *[_ptr(t) for t in (dx, *dw, *db)], M, ldx, lddy, D, F, act,
+                        _DT[x.dtype], ws.data_ptr(), n)
+    _check(lib.fluxhip_gated_ff_grad(d, st), "fluxhip_gated_ff_grad")
     return (dx, *dw, *db)
