@@ -26,17 +26,22 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 enum { EPI_STORE = 0, EPI_UP = 1, EPI_DH = 2 };
 
-struct FfArgs {
+struct FfProd {                 // out[m][n] = sum over segments of Q[seg] P[seg]
   const char *P[2], *Q[2];
-  char* out[2];
-  int64_t ldp, ldq;           // element strides of the operands' rows
-  int64_t ldo;                // ... of the output's rows
-  int M, N, K;                // output rows and columns, contraction length of a segment
-  int nseg, nbatch, splits;   // segments s add P[s] Q[s]; batches b write out[b] = P[0] Q[b]
-  int tiles_m, tiles_n, act;
+  char* out;
+  int64_t ldp, ldq, ldo;        // element strides of the rows of P, Q, out
+  int M, N, tiles_m, tiles_n;
+};
+// One launch: up to three products of one contraction length, their tiles in one list.  The first `full` tiles are whole work
+// items, every tile behind them is `splits` items along k whose partial tiles ff_finish_kernel adds.
+struct FfArgs {
+  FfProd pr[3];
+  int nprod, K, nseg, act;      // K: contraction length of a segment
+  int full, splits, items;
+  float* part;                  // partial tiles of the split items
   const char *bias[2], *value, *gate;
-  char *vout, *gout;          // EPI_UP: saved value / gate (or null); EPI_DH: dvalue / dgate
-  float* part;                // EPI_STORE with splits > 1: partial products; EPI_DH: column sums [2 tiles_m][2][N] (or null)
+  char *vout, *gout;            // EPI_UP: saved value / gate (or null); EPI_DH: dvalue / dgate
+  float* colsum;                // EPI_DH: partial column sums [rows][2][N] (or null)
 };
 
 // gfx950 fragment swizzles.  row tile: 64 k = 8 chunks of 16 bytes a row, chunk ^= (row >> 1) & 7.  col tile: one k a row, its
@@ -174,58 +179,230 @@ DEVINL void swap16(float& a, float& b) {
 
 // NF n and MF m fragments per wave, WN x WM waves; block tile BT = 16 NF WN = 16 MF WM squared, 1 KiB x 4 pieces of either
 // operand per wave and stage.  MF = 8: 256 square, eight waves (two a SIMD); MF = 4: 128 square, four waves, two blocks a CU.
+template <int MF, int EPI>
+struct Geo {
+  static constexpr int NF = 4, BT = 32 * MF, WN = BT / 64, NW = 2 * WN, BN = EPI == EPI_UP ? BT / 2 : BT, OPB = BT * BK * 2, STAGE = 2 * OPB;
+};
+
+struct Item { int p, m0, n0, s_lo, ns, slot; };            // slot: of the partial tile, -1 for a whole one
+template <int MF, int EPI>
+DEVINL Item item_of(const FfArgs& a, int it) {
+  typedef Geo<MF, EPI> G;
+  Item r;
+  const int sps = (a.K + BK - 1) / BK, total = sps * a.nseg;
+  int t = it, split = 0;
+  r.slot = -1;
+  r.s_lo = 0;
+  r.ns = total;
+  if (it >= a.full) {
+    const int u = it - a.full, q = u / a.splits;
+    t = a.full + q;
+    if (a.splits > 1) {
+      split = u - q * a.splits;
+      r.slot = u;
+      r.s_lo = (uint32_t)(total * split) / (uint32_t)a.splits;       // (total <= 2^25, splits <= 16)
+      r.ns = (uint32_t)(total * (split + 1)) / (uint32_t)a.splits - r.s_lo;
+    }
+  }
+  r.p = 0;
+  while (r.p + 1 < a.nprod && t >= a.pr[r.p].tiles_m * a.pr[r.p].tiles_n) t -= a.pr[r.p].tiles_m * a.pr[r.p].tiles_n, ++r.p;
+  // bands of four row tiles: neighbouring items share operand tiles
+  const int tm = a.pr[r.p].tiles_m, tn = a.pr[r.p].tiles_n, band = t / (4 * tn), bm = min(4, tm - band * 4);
+  t -= band * 4 * tn;
+  r.m0 = (band * 4 + t % bm) * G::BT;
+  r.n0 = t / bm * G::BN;
+  return r;
+}
+
+// writes J m fragments of a tile, the first at row mb (this lane's) and column nb (with the lane's offset behind the swap)
+template <int MF, int EPI, bool H, int J>
+DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[4][J], int m0, int n0, int wm, int wn, int j0) {
+  typedef Geo<MF, EPI> G;
+  constexpr int NF = G::NF;
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int nb = n0 + (EPI == EPI_UP ? wn * (NF * 8) : wn * (NF * 16)) + (q & 1) * 16 + (q >> 1) * 8;
+  const int mb = m0 + wm * (MF * 16) + j0 * 16 + c;
+  typedef uint16_t E;
+  typedef Elem<H ? 1 : 0> El;
+  if constexpr (EPI == EPI_UP) {
+    const int n = nb;
+    const bool in = n < pr.N;
+    float bv[8] = {}, bg[8] = {};
+    if (in && a.bias[0]) {
+      El::load8((const E*)a.bias[0] + n, 0, 8, bv);
+      El::load8((const E*)a.bias[1] + n, 0, 8, bg);
+    }
+    static_for<0, J>([&](auto j) {
+      const int m = mb + j * 16;
+      float v[8], g[8], h[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = acc[0][j][e]; v[4 + e] = acc[1][j][e];
+        g[e] = acc[2][j][e]; g[4 + e] = acc[3][j][e];
+        swap16(v[e], v[4 + e]);
+        swap16(g[e], g[4 + e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] += bv[e];
+        g[e] += bg[e];
+        h[e] = v[e] * act_f(g[e], a.act);
+      }
+      if (in && m < pr.M) {
+        const int64_t o = (int64_t)m * pr.N + n;
+        El::store8((E*)pr.out + o, 0, 8, h);
+        if (a.vout) {
+          El::store8((E*)a.vout + o, 0, 8, v);
+          El::store8((E*)a.gout + o, 0, 8, g);
+        }
+      }
+    });
+  } else if constexpr (EPI == EPI_DH) {
+    // the saved value and gate of the items ahead are in flight while one is worked on (addresses behind the ends are clamped,
+    // their results dropped)
+    constexpr int NI = 2 * J, AHEAD = J < 4 ? NI : 4;
+    typename El::raw8 rv[AHEAD], rg[AHEAD];
+    auto fetch = [&](auto k) {
+      const int m = min(mb + (k % J) * 16, pr.M - 1), n = min(nb + (k / J) * 32, pr.N - 8);
+      const int64_t o = (int64_t)m * pr.N + n;
+      El::fetch8((const E*)a.value + o, 0, 8, rv[k % AHEAD]);
+      El::fetch8((const E*)a.gate + o, 0, 8, rg[k % AHEAD]);
+    };
+    static_for<0, AHEAD>([&](auto k) { fetch(k); });
+    static_for<0, 2>([&](auto ih) {
+      constexpr int i = 2 * ih;
+      const int n = nb + i * 16;
+      const bool in = n < pr.N;
+      float sv[8] = {}, sg[8] = {};
+      static_for<0, J>([&](auto j) {
+        constexpr int k = ih * J + j;
+        const int m = mb + j * 16;
+        float d[8], v[8], g[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          d[e] = acc[i][j][e]; d[4 + e] = acc[i + 1][j][e];
+          swap16(d[e], d[4 + e]);
+        }
+        El::open8(rv[k % AHEAD], v);
+        El::open8(rg[k % AHEAD], g);
+        if constexpr (k + AHEAD < NI) fetch(std::integral_constant<int, k + AHEAD>{});
+        const bool ok = in && m < pr.M;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float f, df;
+          act_grad(g[e], a.act, f, df);
+          g[e] = d[e] * v[e] * df;
+          v[e] = d[e] * f;
+          sv[e] += ok ? v[e] : 0.f;
+          sg[e] += ok ? g[e] : 0.f;
+        }
+        if (ok) {
+          const int64_t o = (int64_t)m * pr.N + n;
+          El::store8((E*)a.vout + o, 0, 8, v);
+          El::store8((E*)a.gout + o, 0, 8, g);
+        }
+        // column sums over the wave's rows: 16 lanes in a fixed order; per 32 rows where the launch has split tiles
+        if ((j & 1) && a.colsum && (j == J - 1 || a.splits > 1)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            sv[e] = row16_sum(sv[e]);
+            sg[e] = row16_sum(sg[e]);
+          }
+          if (c == 0 && in) {
+            const int64_t row = (int64_t)(m0 / G::BT) * 2 + wm;
+            float* p = a.colsum + (a.splits > 1 ? row * (MF / 2) + (j0 + j) / 2 : row) * 2 * pr.N + n;
+            Elem<2>::store8(p, 0, 8, sv);
+            Elem<2>::store8(p + pr.N, 0, 8, sg);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sv[e] = sg[e] = 0.f;
+        }
+      });
+    });
+  } else {
+    static_for<0, 2>([&](auto ih) {
+      constexpr int i = 2 * ih;
+      const int n = nb + i * 16;
+      const bool in = n < pr.N;
+      float b[8] = {};
+      if (in && a.bias[0]) El::load8((const E*)a.bias[0] + n, 0, 8, b);
+      static_for<0, J>([&](auto j) {
+        const int m = mb + j * 16;
+        float d[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          d[e] = acc[i][j][e]; d[4 + e] = acc[i + 1][j][e];
+          swap16(d[e], d[4 + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] += b[e];
+        if (in && m < pr.M) El::store8((E*)pr.out + (int64_t)m * pr.ldo + n, 0, 8, d);
+      });
+    });
+  }
+}
+
 template <int MF, bool PC, bool QC, int EPI, bool H>
 __global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs a) {
-  constexpr int NF = 4, BT = 32 * MF, WN = BT / 64, OPB = BT * BK * 2, STAGE = 2 * OPB;   // bytes of an operand tile, of a stage
+  typedef Geo<MF, EPI> G;
+  constexpr int NF = G::NF, BT = G::BT, WN = G::WN, OPB = G::OPB, STAGE = G::STAGE;
   __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / WN, wn = wave % WN;
 
-  // block -> (split, batch, tile): consecutive ids of one XCD (id mod 8) walk bands of four row tiles, so its 32 CUs share
-  // operand tiles in that XCD's L2
-  int id = blockIdx.x;
+  // block -> first item: the blocks of one XCD (id mod 8) take neighbouring items, so its CUs share operand tiles in their L2;
+  // then every gridDim-th
+  int it0 = blockIdx.x;
   {
-    const int n = gridDim.x, per = n >> 3, rem = n & 7, x = id & 7;
-    id = x * per + min(x, rem) + (id >> 3);
+    const int n = gridDim.x, per = n >> 3, rem = n & 7, x = it0 & 7;
+    it0 = x * per + min(x, rem) + (it0 >> 3);
   }
-  const int tiles = a.tiles_m * a.tiles_n;
-  int t = id % tiles;
-  const int z = id / tiles, batch = z % a.nbatch, split = z / a.nbatch;
-  const int band = t / (4 * a.tiles_n), bm = min(4, a.tiles_m - band * 4);
-  t -= band * 4 * a.tiles_n;
-  const int m0 = (band * 4 + t % bm) * BT;
-  const int tn = t / bm, n0 = tn * (EPI == EPI_UP ? BT / 2 : BT);
 
-  const int sps = (a.K + BK - 1) / BK, total = sps * a.nseg;
-  const int s_lo = (int)((int64_t)total * split / a.splits), s_hi = (int)((int64_t)total * (split + 1) / a.splits), ns = s_hi - s_lo;
-
+  // ---- what is being fetched: a stream of steps that runs two ahead of the products, across items
   // EPI_UP: P is two half tiles, value rows then gate rows, staged by the first and the second half of the waves
-  Stager<PC, EPI == EPI_UP ? BT / 2 : BT> sp;
+  Stager<PC, G::BN> sp;
   Stager<QC, BT> sq;
-  const char *pbase[2] = {a.P[0], a.P[1]}, *qbase[2] = {a.nbatch > 1 ? a.Q[batch] : a.Q[0], a.Q[1]};
-  if (EPI == EPI_UP && wave >= WN) pbase[0] = a.P[1];      // (WN is half the number of waves)
-  sp.init(lane, (EPI == EPI_UP ? wave % WN : wave) * 4, a.ldp, n0, a.N, a.K);
-  sq.init(lane, wave * 4, a.ldq, m0, a.M, a.K);
-  Reader<PC, BT> rp;
-  Reader<QC, BT> rq;
-  rp.init(lane);
-  rq.init(lane);
-
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 4096;
-  auto open = [&](int s) {                                 // resources of step s
-    const bool on = s < ns;                                // behind the last step: empty resources, the pieces write zeros
-    const int st = s_lo + s, seg = a.nseg > 1 && st >= sps ? 1 : 0, k0 = (st - seg * sps) * BK;
-    sp.step(pbase[EPI == EPI_UP ? 0 : seg], k0, on);
-    sq.step(qbase[seg], k0, on);
+  int f_it = it0, f_s = 0, f_ns = 0, f_lo = 0;
+  const char *pb[2], *qb[2];
+  const int sps = (a.K + BK - 1) / BK;
+  auto f_item = [&]() {
+    const Item r = item_of<MF, EPI>(a, f_it);
+    const FfProd& pr = a.pr[r.p];
+    f_s = 0;
+    f_ns = r.ns;
+    f_lo = r.s_lo;
+    pb[0] = EPI == EPI_UP && wave >= WN ? pr.P[1] : pr.P[0];   // (WN is half the number of waves)
+    pb[1] = pr.P[1];
+    qb[0] = pr.Q[0];
+    qb[1] = pr.Q[1];
+    sp.init(lane, (EPI == EPI_UP ? wave % WN : wave) * 4, pr.ldp, r.n0, pr.N, a.K);
+    sq.init(lane, wave * 4, pr.ldq, r.m0, pr.M, a.K);
   };
+  f_item();
+  auto open = [&]() {                                      // resources of the stream's next step
+    if (f_s == f_ns && f_it < a.items) {
+      f_it += gridDim.x;
+      if (f_it < a.items) f_item();
+    }
+    const bool on = f_it < a.items;                        // behind the last step: empty resources, the pieces write zeros
+    const int st = f_lo + f_s, seg = a.nseg > 1 && st >= sps ? 1 : 0, k0 = (st - seg * sps) * BK;
+    sp.step(seg ? pb[1] : pb[0], k0, on);
+    sq.step(seg ? qb[1] : qb[0], k0, on);
+    f_s += on ? 1 : 0;
+  };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 4096;
   auto piece = [&](int j, int buf) {                       // j-th of the wave's 8 pieces of a stage
     const uint32_t d = lds0 + buf * STAGE;
     if (j < 4) sp.piece(j, d);
     else sq.piece(j - 4, d + OPB);
   };
 
+  // ---- products
+  Reader<PC, BT> rp;
+  Reader<QC, BT> rq;
+  rp.init(lane);
+  rq.init(lane);
   f32x4 acc[NF][MF];                                       // [n fragment][m fragment]
-  static_for<0, NF>([&](auto i) { static_for<0, MF>([&](auto j) { acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}; }); });
   bf16x8 fp[2][NF], fq[MF];
   auto read_p = [&](int i, int buf, int ks) {              // fragments of k half ks of a stage
     const int row = EPI == EPI_UP ? (i >= NF / 2 ? BT / 2 : 0) + wn * (NF * 8) + (i % (NF / 2)) * 16 : wn * (NF * 16) + i * 16;
@@ -240,26 +417,29 @@ __global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
   // fragment it used is free and is read for the next half (P fragments alternate between two sets), so every LDS read has
   // about MF groups to land.  Once per step, behind the first group of the second half (it covers the last reads' latency),
   // the waves meet: all have the stage in registers and all pieces of the next stage are in LDS; the stage is then refilled
-  // with step s + 2, whose loads have a whole step to land.
-  if (ns > 0) {
-    open(0);
-    static_for<0, 8>([&](auto j) { piece(j, 0); });
-    open(1);
-    static_for<0, 8>([&](auto j) { piece(j, 1); });
-    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    static_for<0, NF>([&](auto i) { read_p(i, 0, 0); });
-    static_for<0, MF>([&](auto j) { read_q(j, 0, 0); });
-    for (int s = 0; s < ns; ++s) {
-      const int buf = s & 1;
+  // with the step after the next, whose loads have a whole step to land.  The stream does not stop at an item's end: the next
+  // item's first stages land while this one's tile is written.
+  open();
+  static_for<0, 8>([&](auto j) { piece(j, 0); });
+  open();
+  static_for<0, 8>([&](auto j) { piece(j, 1); });
+  asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  int buf = 0;
+  for (int it = it0; it < a.items; it += gridDim.x) {
+    const Item r = item_of<MF, EPI>(a, it);
+    static_for<0, NF>([&](auto i) { read_p(i, buf, 0); });   // (read again behind an epilogue: it needs the registers)
+    static_for<0, MF>([&](auto j) { read_q(j, buf, 0); });
+    static_for<0, NF>([&](auto i) { static_for<0, MF>([&](auto j) { acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}; }); });
+    for (int s = 0; s < r.ns; ++s) {
       static_for<0, MF>([&](auto j) {
         mul(j, 0);
         read_q(j, buf, 1);
         if constexpr (j < NF) read_p(j, buf, 1);
         __builtin_amdgcn_sched_barrier(0);
       });
-      open(s + 2);
+      open();
       static_for<0, MF>([&](auto j) {
         mul(j, 1);
         if constexpr (j == 0) {
@@ -269,219 +449,150 @@ __global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
           asm volatile("" ::: "memory");
         }
         static_for<j * 8 / MF, (j + 1) * 8 / MF>([&](auto e) { piece(e, buf); });
-        read_q(j, buf ^ 1, 0);                             // (behind the last step: a stale stage, in bounds and not used)
+        read_q(j, buf ^ 1, 0);                             // (behind the very last step: zeros, not used)
         if constexpr (j < NF) read_p(j, buf ^ 1, 0);
         __builtin_amdgcn_sched_barrier(0);
       });
+      buf ^= 1;
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no piece outlives the loop
+    if (r.slot >= 0) {                                     // a partial tile, fragments as they lie in the registers
+      f32x4* p = (f32x4*)a.part + (((int64_t)r.slot * G::NW + wave) * (NF * MF)) * 64 + lane;
+      static_for<0, NF>([&](auto i) { static_for<0, MF>([&](auto j) { p[(i * MF + j) * 64] = acc[i][j]; }); });
+    } else {
+      epilogue<MF, EPI, H, MF>(a, a.pr[r.p], acc, r.m0, r.n0, wm, wn, 0);
+    }
   }
-
-  // ---- epilogue: lane holds m = .. + (lane & 15); after the swap 8 neighbouring n
-  const int c = lane & 15, q = lane >> 4, noff = (q & 1) * 16 + (q >> 1) * 8;
-  const int nb = n0 + (EPI == EPI_UP ? wn * (NF * 8) : wn * (NF * 16)) + noff, mb = m0 + wm * (MF * 16) + c;
-  typedef uint16_t E;
-  typedef Elem<H ? 1 : 0> El;
-  if constexpr (EPI == EPI_UP) {
-    static_for<0, NF / 4>([&](auto ih) {
-      constexpr int i = 2 * ih;
-      const int n = nb + i * 16;
-      const bool in = n < a.N;
-      float bv[8] = {}, bg[8] = {};
-      if (in && a.bias[0]) {
-        El::load8((const E*)a.bias[0] + n, 0, 8, bv);
-        El::load8((const E*)a.bias[1] + n, 0, 8, bg);
-      }
-      static_for<0, MF>([&](auto j) {
-        const int m = mb + j * 16;
-        float v[8], g[8], h[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = acc[i][j][e]; v[4 + e] = acc[i + 1][j][e];
-          g[e] = acc[i + NF / 2][j][e]; g[4 + e] = acc[i + 1 + NF / 2][j][e];
-          swap16(v[e], v[4 + e]);
-          swap16(g[e], g[4 + e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] += bv[e];
-          g[e] += bg[e];
-          h[e] = v[e] * act_f(g[e], a.act);
-        }
-        if (in && m < a.M) {
-          const int64_t o = (int64_t)m * a.N;
-          El::store8((E*)a.out[0] + o + n, 0, 8, h);
-          if (a.vout) {
-            El::store8((E*)a.vout + o + n, 0, 8, v);
-            El::store8((E*)a.gout + o + n, 0, 8, g);
-          }
-        }
-      });
-    });
-  } else if constexpr (EPI == EPI_DH) {
-    static_for<0, NF / 2>([&](auto ih) {
-      constexpr int i = 2 * ih;
-      const int n = nb + i * 16;
-      const bool in = n < a.N;
-      float sv[8] = {}, sg[8] = {};
-      static_for<0, MF>([&](auto j) {
-        const int m = mb + j * 16;
-        float d[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d[e] = acc[i][j][e]; d[4 + e] = acc[i + 1][j][e];
-          swap16(d[e], d[4 + e]);
-        }
-        if (in && m < a.M) {
-          const int64_t o = (int64_t)m * a.N;
-          float v[8], g[8];
-          El::load8((const E*)a.value + o + n, 0, 8, v);
-          El::load8((const E*)a.gate + o + n, 0, 8, g);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float f, df;
-            act_grad(g[e], a.act, f, df);
-            g[e] = d[e] * v[e] * df;
-            v[e] = d[e] * f;
-            sv[e] += v[e];
-            sg[e] += g[e];
-          }
-          El::store8((E*)a.vout + o + n, 0, 8, v);
-          El::store8((E*)a.gout + o + n, 0, 8, g);
-        }
-      });
-      if (a.part) {                                        // column sums over the wave's rows: 16 lanes, fixed order
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sv[e] = row16_sum(sv[e]);
-          sg[e] = row16_sum(sg[e]);
-        }
-        if (c == 0 && in) {
-          float* p = a.part + (int64_t)((m0 / BT) * 2 + wm) * 2 * a.N;
-          Elem<2>::store8(p + n, 0, 8, sv);
-          Elem<2>::store8(p + a.N + n, 0, 8, sg);
-        }
-      }
-    });
-  } else {
-    static_for<0, NF / 2>([&](auto ih) {
-      constexpr int i = 2 * ih;
-      const int n = nb + i * 16;
-      const bool in = n < a.N;
-      float b[8] = {};
-      if (in && a.bias[0] && a.splits == 1) El::load8((const E*)a.bias[0] + n, 0, 8, b);
-      static_for<0, MF>([&](auto j) {
-        const int m = mb + j * 16;
-        float d[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d[e] = acc[i][j][e]; d[4 + e] = acc[i + 1][j][e];
-          swap16(d[e], d[4 + e]);
-        }
-        if (in && m < a.M) {
-          if (a.splits > 1) {
-            Elem<2>::store8(a.part + (((int64_t)split * a.nbatch + batch) * a.M + m) * a.N + n, 0, 8, d);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] += b[e];
-            El::store8((E*)a.out[batch] + (int64_t)m * a.ldo + n, 0, 8, d);
-          }
-        }
-      });
-    });
-  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no piece outlives the kernel
 }
 
-// adds the split-K partial products in split order (+ bias), eight neighbouring columns a thread
-template <bool H>
-__global__ __launch_bounds__(256) void ff_reduce_kernel(FfArgs a) {
-  typedef Elem<H ? 1 : 0> El;
-  const int64_t n8 = a.N / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x, batch = blockIdx.y;
-  if (i >= n8 * a.M) return;
-  const int64_t m = i / n8;
-  const int n = (int)(i - m * n8) * 8;
-  float s[8] = {}, v[8];
-  if (a.bias[0]) El::load8((const uint16_t*)a.bias[0] + n, 0, 8, s);
+// adds a split tile's partials in split order and writes it; a block takes two m fragments of each wave's tile
+template <int MF, int EPI, bool H>
+__global__ __launch_bounds__(MF == 8 ? 512 : 256) void ff_finish_kernel(FfArgs a) {
+  typedef Geo<MF, EPI> G;
+  constexpr int NF = G::NF;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int tile = blockIdx.x / (MF / 2), j0 = blockIdx.x % (MF / 2) * 2;
+  const Item r = item_of<MF, EPI>(a, a.full + tile * a.splits);
+  f32x4 acc[NF][2];
+  static_for<0, NF>([&](auto i) { acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f}; });
+  const f32x4* p = (const f32x4*)a.part + (((int64_t)tile * a.splits * G::NW + wave) * (NF * MF) + j0) * 64 + lane;
+#pragma unroll 2
   for (int z = 0; z < a.splits; ++z) {
-    Elem<2>::load8(a.part + (((int64_t)z * a.nbatch + batch) * a.M + m) * a.N + n, 0, 8, v);
-    for (int e = 0; e < 8; ++e) s[e] += v[e];
+    static_for<0, NF>([&](auto i) {
+      acc[i][0] += p[i * MF * 64];
+      acc[i][1] += p[(i * MF + 1) * 64];
+    });
+    p += (int64_t)G::NW * (NF * MF) * 64;
   }
-  El::store8((uint16_t*)a.out[batch] + m * a.ldo + n, 0, 8, s);
+  epilogue<MF, EPI, H, 2>(a, a.pr[r.p], acc, r.m0, r.n0, wave / G::WN, wave % G::WN, j0);
 }
 
-// column sums of [M][N] (first stage; colsum.h adds the partial rows): block = 2048 columns x a range of rows
+// column sums of [M][N] (first stage; colsum.h adds the partial rows): a wave takes 512 columns of every gridDim.y-th row
 template <bool H>
-__global__ __launch_bounds__(256) void ff_colsum_kernel(const uint16_t* x, int64_t ld, int M, int N, float* part) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
+__global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_t ld, int M, int N, float* part) {
+  typedef Elem<H ? 1 : 0> El;
+  const int c = (blockIdx.x * 64 + threadIdx.x) * 8;
   if (c >= N) return;
   float s[8] = {}, v[8];
-#pragma unroll 4
+#pragma unroll 8
   for (int m = blockIdx.y; m < M; m += gridDim.y) {
-    Elem<H ? 1 : 0>::load8(x + m * ld, c, N, v);
+    El::load8(x + m * ld + c, 0, 8, v);
     for (int e = 0; e < 8; ++e) s[e] += v[e];
   }
-  Elem<2>::store8(part + (int64_t)blockIdx.y * N, c, N, s);
+  Elem<2>::store8(part + (int64_t)blockIdx.y * N + c, 0, 8, s);
 }
 
-struct Plan { int mf, splits; };
-// Tile and split of an [M][N] product of `steps` k-steps (nb batches).  256-square tiles (one block a CU) where they fill the
-// chip, else 128-square ones (two a CU); a product of few tiles is split along k, its partials added by ff_reduce_kernel.
-Plan pick(int64_t M, int64_t N, int nb, int64_t steps, bool can_split) {
-  auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b) * nb; };
-  const int64_t t256 = tiles(256), t128 = tiles(128);
-  if (t256 >= 200) return {8, 1};
-  int splits = 1;
-  if (can_split)
-    while (t128 * splits < 384 && steps / (splits * 2) >= 4 && splits < 16) splits *= 2;
-  return {4, splits};
+// How a launch is cut.  256-square tiles run one block a CU at about 1.5 us a step (64 k) of all CUs, 128-square ones two a CU at
+// 1.13 us (16384 x 5120 x 1280 and 512 x 20480 x 4096, bf16).  Whole rounds of tiles run as they are; the tiles of the last,
+// broken round are split along k over the idle CUs where that pays for writing and reading their float32 partials (0.117 us a
+// 256-square split tile at 4.5 TB/s over the chip, and 5 us for the second launch).
+struct Plan { int mf, full, splits, items; };
+struct Dims { int64_t M, N; };                             // output of a product; EPI_UP: N = F
+Plan pick(const Dims* d, int n, int64_t steps, int epi) {
+  Plan best{};
+  double least = 1e30;
+  for (int mf = 8; mf >= 4; mf -= 4) {
+    const int64_t bt = 32 * mf, bn = epi == EPI_UP ? bt / 2 : bt, slots = mf == 8 ? 256 : 512;
+    const double step = mf == 8 ? 1.5 : 1.13, part = mf == 8 ? 0.117 : 0.029;
+    int64_t tiles = 0;
+    for (int i = 0; i < n; ++i) tiles += ((d[i].M + bt - 1) / bt) * ((d[i].N + bn - 1) / bn);
+    const int64_t full = tiles / slots * slots, tail = tiles - full;
+    for (int64_t s = 1; s <= 16 && s <= steps; ++s) {
+      const double us = step * steps * ((double)(full / slots) + (double)((tail * s + slots - 1) / slots) / s) + (s > 1 ? 5 + tail * s * part : 0);
+      if (us < least) {
+        least = us;
+        best = {mf, (int)full, (int)s, (int)(full + tail * s)};
+      }
+      if (!tail) break;
+    }
+  }
+  return best;
 }
-int64_t part_bytes(int64_t M, int64_t N, int nb, Plan p) { return p.splits > 1 ? M * N * nb * p.splits * 4 : 0; }
-constexpr int COLSUM_ROWS = 256;
+int64_t part_bytes(const Plan& p) { return p.splits > 1 ? (int64_t)(p.items - p.full) * (32 * p.mf) * (32 * p.mf) * 4 : 0; }
 
 template <int MF, bool PC, bool QC, int EPI, bool H>
-void launch_mf(FfArgs& a, hipStream_t st) {
-  constexpr int BT = 32 * MF, BN = EPI == EPI_UP ? BT / 2 : BT;
-  a.tiles_m = (a.M + BT - 1) / BT;
-  a.tiles_n = (a.N + BN - 1) / BN;
-  hipLaunchKernelGGL((ff_gemm_kernel<MF, PC, QC, EPI, H>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.nbatch * a.splits)), dim3(MF == 8 ? 512 : 256), 0,
-                     st, a);
+void launch_mf(FfArgs& a, const Plan& p, hipStream_t st) {
+  typedef Geo<MF, EPI> G;
+  constexpr int slots = MF == 8 ? 256 : 512;
+  for (int i = 0; i < a.nprod; ++i) {
+    a.pr[i].tiles_m = (a.pr[i].M + G::BT - 1) / G::BT;
+    a.pr[i].tiles_n = (a.pr[i].N + G::BN - 1) / G::BN;
+  }
+  hipLaunchKernelGGL((ff_gemm_kernel<MF, PC, QC, EPI, H>), dim3(p.items < slots ? p.items : slots), dim3(G::NW * 64), 0, st, a);
+  if (p.splits > 1)
+    hipLaunchKernelGGL((ff_finish_kernel<MF, EPI, H>), dim3((p.items - p.full) / p.splits * (MF / 2)), dim3(G::NW * 64), 0, st, a);
 }
 template <bool PC, bool QC, int EPI, bool H>
-void launch(FfArgs& a, Plan p, hipStream_t st) {
+void launch(FfArgs& a, const Plan& p, hipStream_t st) {
+  a.full = p.full;
   a.splits = p.splits;
-  if (p.mf == 8) launch_mf<8, PC, QC, EPI, H>(a, st);
-  else launch_mf<4, PC, QC, EPI, H>(a, st);
-  if (EPI == EPI_STORE && a.splits > 1)
-    hipLaunchKernelGGL((ff_reduce_kernel<H>), dim3((unsigned)(((int64_t)a.M * (a.N / 8) + 255) / 256), a.nbatch), dim3(256), 0, st, a);
+  a.items = p.items;
+  if (p.mf == 8) launch_mf<8, PC, QC, EPI, H>(a, p, st);
+  else launch_mf<4, PC, QC, EPI, H>(a, p, st);
 }
 
 int64_t steps_of(int64_t k) { return (k + BK - 1) / BK; }
-Plan plan_up(int64_t M, int D, int F) { return pick(M, 2 * (int64_t)F, 1, steps_of(D), false); }
-Plan plan_down(int64_t M, int D, int F) { return pick(M, D, 1, steps_of(F), true); }
-Plan plan_dh(int64_t M, int D, int F) { return pick(M, F, 1, steps_of(D), false); }
-Plan plan_dx(int64_t M, int D, int F) { return pick(M, D, 1, 2 * steps_of(F), true); }
-Plan plan_dwo(int64_t M, int D, int F) { return pick(D, F, 1, steps_of(M), true); }
-Plan plan_dwv(int64_t M, int D, int F) { return pick(F, D, 2, steps_of(M), true); }
+Plan plan_up(int64_t M, int D, int F) { const Dims d{M, F}; return pick(&d, 1, steps_of(D), EPI_UP); }
+Plan plan_down(int64_t M, int D, int F) { const Dims d{M, D}; return pick(&d, 1, steps_of(F), EPI_STORE); }
+Plan plan_dh(int64_t M, int D, int F) { const Dims d{M, F}; return pick(&d, 1, steps_of(D), EPI_DH); }
+Plan plan_dx(int64_t M, int D, int F) { const Dims d{M, D}; return pick(&d, 1, 2 * steps_of(F), EPI_STORE); }
+Plan plan_dw(int64_t M, int D, int F) { const Dims d[3] = {{F, D}, {F, D}, {D, F}}; return pick(d, 3, steps_of(M), EPI_STORE); }
+Plan plan_dw2(int64_t M, int D, int F) { const Dims d[2] = {{F, D}, {F, D}}; return pick(d, 2, steps_of(M), EPI_STORE); }
+Plan plan_dw1(int64_t M, int D, int F) { const Dims d{D, F}; return pick(&d, 1, steps_of(M), EPI_STORE); }
+int64_t colsum_rows(int64_t M, const Plan& p) { return (M + 32 * p.mf - 1) / (32 * p.mf) * 2 * (p.splits > 1 ? p.mf / 2 : 1); }
+constexpr int COLSUM_ROWS = 512;
 
 bool bad(int64_t M, int D, int F, int act, int dtype) {
   return M < 0 || M > (1 << 30) || D < 8 || F < 8 || D % 8 || F % 8 || D > (1 << 20) || F > (1 << 20) || dtype < 0 || dtype > 1 ||
+         (M / 128 + 1) * ((D > F ? D : F) / 64 + 1) > (1 << 30) ||       // (tiles are counted in 32 bits)
          (act != FLUXHIP_EPI_GELU_TANH && act != FLUXHIP_EPI_GELU_ERF && act != FLUXHIP_EPI_SILU);
 }
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
+FfProd prod(const void* P, const void* Q, void* out, int64_t ldp, int64_t ldq, int64_t ldo, int64_t M, int64_t N) {
+  FfProd r{};
+  r.P[0] = r.P[1] = (const char*)P;
+  r.Q[0] = r.Q[1] = (const char*)Q;
+  r.out = (char*)out;
+  r.ldp = ldp; r.ldq = ldq; r.ldo = ldo; r.M = (int)M; r.N = (int)N;
+  return r;
+}
+
 template <bool H>
 void forward(const fluxhip_gated_ff_desc* d, hipStream_t st) {
+  const int64_t M = d->M;
+  const int D = d->D, F = d->F;
   FfArgs a{};
-  a.P[0] = (const char*)d->w_value; a.P[1] = (const char*)d->w_gate; a.Q[0] = a.Q[1] = (const char*)d->x;
-  a.out[0] = (char*)d->hidden; a.vout = (char*)d->value; a.gout = (char*)d->gate;
+  a.pr[0] = prod(d->w_value, d->x, d->hidden, D, d->ldx, F, M, F);
+  a.pr[0].P[1] = (const char*)d->w_gate;
+  a.nprod = a.nseg = 1; a.K = D; a.act = d->act; a.part = (float*)d->ws;
+  a.vout = (char*)d->value; a.gout = (char*)d->gate;
   a.bias[0] = (const char*)d->b_value; a.bias[1] = (const char*)d->b_gate;
-  a.ldp = d->D; a.ldq = d->ldx; a.M = (int)d->M; a.N = d->F; a.K = d->D; a.nseg = a.nbatch = 1; a.act = d->act;
-  launch<false, false, EPI_UP, H>(a, plan_up(d->M, d->D, d->F), st);
+  launch<false, false, EPI_UP, H>(a, plan_up(M, D, F), st);
   FfArgs b{};
-  b.P[0] = b.P[1] = (const char*)d->w_out; b.Q[0] = b.Q[1] = (const char*)d->hidden; b.out[0] = (char*)d->y;
-  b.bias[0] = (const char*)d->b_out;
-  b.ldp = b.ldq = d->F; b.ldo = d->D; b.M = (int)d->M; b.N = d->D; b.K = d->F; b.nseg = b.nbatch = 1; b.part = (float*)d->ws;
-  launch<false, false, EPI_STORE, H>(b, plan_down(d->M, d->D, d->F), st);
+  b.pr[0] = prod(d->w_out, d->hidden, d->y, F, F, D, M, D);
+  b.nprod = b.nseg = 1; b.K = F; b.part = (float*)d->ws; b.bias[0] = (const char*)d->b_out;
+  launch<false, false, EPI_STORE, H>(b, plan_down(M, D, F), st);
 }
 
 template <bool H>
@@ -489,38 +600,39 @@ void backward(const fluxhip_gated_ff_grad_desc* d, hipStream_t st) {
   const int64_t M = d->M;
   const int D = d->D, F = d->F;
   {
+    const Plan p = plan_dh(M, D, F);
     FfArgs a{};
-    a.P[0] = a.P[1] = (const char*)d->w_out; a.Q[0] = a.Q[1] = (const char*)d->dy;
+    a.pr[0] = prod(d->w_out, d->dy, nullptr, F, d->lddy, F, M, F);
+    a.nprod = a.nseg = 1; a.K = D; a.act = d->act;
     a.value = (const char*)d->value; a.gate = (const char*)d->gate; a.vout = (char*)d->dvalue; a.gout = (char*)d->dgate;
-    a.ldp = F; a.ldq = d->lddy; a.M = (int)M; a.N = F; a.K = D; a.nseg = a.nbatch = 1; a.act = d->act;
-    a.part = d->db_value ? (float*)d->ws : nullptr;
-    launch<true, false, EPI_DH, H>(a, plan_dh(M, D, F), st);
+    a.part = (float*)((char*)d->ws + (d->db_value ? colsum_rows(M, p) * 2 * F * 4 : 0));
+    a.colsum = d->db_value ? (float*)d->ws : nullptr;
+    launch<true, false, EPI_DH, H>(a, p, st);
     if (d->db_value) {
-      launch_colsum_final(a.part, 2 * a.tiles_m, 1, 2, F, d->db_value, d->db_gate, H ? 1 : 0, st);
+      launch_colsum_final(a.colsum, colsum_rows(M, p), 1, 2, F, d->db_value, d->db_gate, H ? 1 : 0, st);
       const int rows = (int)(M < COLSUM_ROWS ? M : COLSUM_ROWS);
-      hipLaunchKernelGGL((ff_colsum_kernel<H>), dim3((D + 2047) / 2048, rows), dim3(256), 0, st, (const uint16_t*)d->dy, d->lddy, (int)M, D,
+      hipLaunchKernelGGL((ff_colsum_kernel<H>), dim3((D + 511) / 512, rows), dim3(64), 0, st, (const uint16_t*)d->dy, d->lddy, (int)M, D,
                          (float*)d->ws);
       launch_colsum_final((const float*)d->ws, rows, 1, 1, D, d->db_out, nullptr, H ? 1 : 0, st);
     }
   }
   if (d->dx) {
     FfArgs a{};
-    a.P[0] = (const char*)d->w_value; a.P[1] = (const char*)d->w_gate; a.Q[0] = (const char*)d->dvalue; a.Q[1] = (const char*)d->dgate;
-    a.out[0] = (char*)d->dx; a.ldp = D; a.ldq = F; a.ldo = D; a.M = (int)M; a.N = D; a.K = F; a.nseg = 2; a.nbatch = 1; a.part = (float*)d->ws;
+    a.pr[0] = prod(d->w_value, d->dvalue, d->dx, D, F, D, M, D);
+    a.pr[0].P[1] = (const char*)d->w_gate;
+    a.pr[0].Q[1] = (const char*)d->dgate;
+    a.nprod = 1; a.nseg = 2; a.K = F; a.part = (float*)d->ws;
     launch<true, false, EPI_STORE, H>(a, plan_dx(M, D, F), st);
   }
-  if (d->dw_value) {
+  if (d->dw_value || d->dw_out) {                          // all weight gradients in one launch
     FfArgs a{};
-    a.P[0] = a.P[1] = (const char*)d->x; a.Q[0] = (const char*)d->dvalue; a.Q[1] = (const char*)d->dgate;
-    a.out[0] = (char*)d->dw_value; a.out[1] = (char*)d->dw_gate;
-    a.ldp = d->ldx; a.ldq = F; a.ldo = D; a.M = F; a.N = D; a.K = (int)M; a.nseg = 1; a.nbatch = 2; a.part = (float*)d->ws;
-    launch<true, true, EPI_STORE, H>(a, plan_dwv(M, D, F), st);
-  }
-  if (d->dw_out) {
-    FfArgs a{};
-    a.P[0] = a.P[1] = (const char*)d->hidden; a.Q[0] = a.Q[1] = (const char*)d->dy; a.out[0] = (char*)d->dw_out;
-    a.ldp = F; a.ldq = d->lddy; a.ldo = F; a.M = D; a.N = F; a.K = (int)M; a.nseg = a.nbatch = 1; a.part = (float*)d->ws;
-    launch<true, true, EPI_STORE, H>(a, plan_dwo(M, D, F), st);
+    if (d->dw_value) {
+      a.pr[a.nprod++] = prod(d->x, d->dvalue, d->dw_value, d->ldx, F, D, F, D);
+      a.pr[a.nprod++] = prod(d->x, d->dgate, d->dw_gate, d->ldx, F, D, F, D);
+    }
+    if (d->dw_out) a.pr[a.nprod++] = prod(d->hidden, d->dy, d->dw_out, F, d->lddy, F, D, F);
+    a.nseg = 1; a.K = (int)M; a.part = (float*)d->ws;
+    launch<true, true, EPI_STORE, H>(a, a.nprod == 3 ? plan_dw(M, D, F) : a.nprod == 2 ? plan_dw2(M, D, F) : plan_dw1(M, D, F), st);
   }
 }
 
@@ -530,14 +642,15 @@ int64_t most(int64_t a, int64_t b) { return a > b ? a : b; }
 
 extern "C" int64_t fluxhip_gated_ff_ws(int64_t M, int D, int F) {
   if (bad(M, D, F, FLUXHIP_EPI_SILU, 0)) return FLUXHIP_EINVAL;
-  return part_bytes(M, D, 1, plan_down(M, D, F));
+  return most(part_bytes(plan_up(M, D, F)), part_bytes(plan_down(M, D, F)));
 }
 extern "C" int64_t fluxhip_gated_ff_grad_ws(int64_t M, int D, int F) {
   if (bad(M, D, F, FLUXHIP_EPI_SILU, 0)) return FLUXHIP_EINVAL;
-  int64_t b = most(((M + 127) / 128) * 2 * 2 * (int64_t)F * 4, (int64_t)COLSUM_ROWS * D * 4);
-  b = most(b, part_bytes(M, D, 1, plan_dx(M, D, F)));
-  b = most(b, part_bytes(F, D, 2, plan_dwv(M, D, F)));
-  return most(b, part_bytes(D, F, 1, plan_dwo(M, D, F)));
+  const Plan dh = plan_dh(M, D, F);
+  int64_t b = most(colsum_rows(M, dh) * 2 * F * 4 + part_bytes(dh), (int64_t)COLSUM_ROWS * D * 4);
+  b = most(b, part_bytes(plan_dx(M, D, F)));
+  b = most(b, most(part_bytes(plan_dw(M, D, F)), part_bytes(plan_dw2(M, D, F))));
+  return most(b, part_bytes(plan_dw1(M, D, F)));
 }
 
 extern "C" int fluxhip_gated_ff(const fluxhip_gated_ff_desc* d, void* stream) {
