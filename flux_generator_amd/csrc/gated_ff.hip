@@ -177,17 +177,19 @@ DEVINL void swap16(float& a, float& b) {
   b = __uint_as_float(r[1]);
 }
 
-// NF n and MF m fragments per wave, WN x WM waves; block tile BT = 16 NF WN = 16 MF WM squared, 1 KiB x 4 pieces of either
-// operand per wave and stage.  MF = 8: 256 square, eight waves (two a SIMD); MF = 4: 128 square, four waves, two blocks a CU.
-template <int MF, int EPI>
+// A wave's tile is NF n by MF m fragments of 16 (128 or 64 columns - long pieces of output rows - by 64 rows), the block's 2 x WM
+// waves; block tile BT squared, 4 pieces of 1 KiB of either operand per wave and stage.  NF = 8: 256 square, eight waves (two a
+// SIMD); NF = 4: 128 square, four waves, two blocks a CU.
+template <int NF, int EPI>
 struct Geo {
-  static constexpr int NF = 4, BT = 32 * MF, WN = BT / 64, NW = 2 * WN, BN = EPI == EPI_UP ? BT / 2 : BT, OPB = BT * BK * 2, STAGE = 2 * OPB;
+  static constexpr int MF = 4, BT = 32 * NF, WN = 2, WM = BT / 64, NW = WN * WM, BN = EPI == EPI_UP ? BT / 2 : BT, OPB = BT * BK * 2,
+                       STAGE = 2 * OPB;
 };
 
 struct Item { int p, m0, n0, s_lo, ns, slot; };            // slot: of the partial tile, -1 for a whole one
-template <int MF, int EPI>
+template <int NF, int EPI>
 DEVINL Item item_of(const FfArgs& a, int it) {
-  typedef Geo<MF, EPI> G;
+  typedef Geo<NF, EPI> G;
   Item r;
   const int sps = (a.K + BK - 1) / BK, total = sps * a.nseg;
   int t = it, split = 0;
@@ -214,141 +216,144 @@ DEVINL Item item_of(const FfArgs& a, int it) {
   return r;
 }
 
-// writes J m fragments of a tile, the first at row mb (this lane's) and column nb (with the lane's offset behind the swap)
-template <int MF, int EPI, bool H, int J>
-DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[4][J], int m0, int n0, int wm, int wn, int j0) {
-  typedef Geo<MF, EPI> G;
-  constexpr int NF = G::NF;
+// writes J m fragments of a wave's tile, from the j0-th.  Rows outside, their columns inside: one row's pieces (of one or several
+// tensors) are written together, which keeps the pages in reach of the CU's TLB (dvalue / dgate of 16384 x 5120: 372 -> 325 us
+// against the other order).
+template <int NF, int EPI, bool H, int J>
+DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int m0, int n0, int wm, int wn, int j0) {
+  typedef Geo<NF, EPI> G;
+  constexpr int HALVES = EPI == EPI_UP ? NF / 4 : NF / 2;  // pairs of fragments = 32 columns
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int nb = n0 + (EPI == EPI_UP ? wn * (NF * 8) : wn * (NF * 16)) + (q & 1) * 16 + (q >> 1) * 8;
-  const int mb = m0 + wm * (MF * 16) + j0 * 16 + c;
+  const int nb = n0 + wn * (HALVES * 32) + (q & 1) * 16 + (q >> 1) * 8;    // the lane's 8 columns behind the swap
+  const int mb = m0 + wm * (G::MF * 16) + j0 * 16 + c;
   typedef uint16_t E;
   typedef Elem<H ? 1 : 0> El;
-  if constexpr (EPI == EPI_UP) {
-    const int n = nb;
-    const bool in = n < pr.N;
-    float bv[8] = {}, bg[8] = {};
-    if (in && a.bias[0]) {
-      El::load8((const E*)a.bias[0] + n, 0, 8, bv);
-      El::load8((const E*)a.bias[1] + n, 0, 8, bg);
+  auto take = [&](auto i, auto j, float (&d)[8]) {         // fragments i, i + 1 -> 8 neighbouring n
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      d[e] = acc[i][j][e];
+      d[4 + e] = acc[i + 1][j][e];
+      swap16(d[e], d[4 + e]);
     }
+  };
+  if constexpr (EPI == EPI_UP) {
     static_for<0, J>([&](auto j) {
-      const int m = mb + j * 16;
-      float v[8], g[8], h[8];
+      static_for<0, HALVES>([&](auto ih) {
+        const int m = mb + j * 16, n = nb + ih * 32;
+        float v[8], g[8], h[8];
+        take(std::integral_constant<int, 2 * ih>{}, j, v);
+        take(std::integral_constant<int, 2 * ih + NF / 2>{}, j, g);
+        if (n < pr.N && m < pr.M) {
+          if (a.bias[0]) {
+            El::load8((const E*)a.bias[0] + n, 0, 8, h);
+            for (int e = 0; e < 8; ++e) v[e] += h[e];
+            El::load8((const E*)a.bias[1] + n, 0, 8, h);
+            for (int e = 0; e < 8; ++e) g[e] += h[e];
+          }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = acc[0][j][e]; v[4 + e] = acc[1][j][e];
-        g[e] = acc[2][j][e]; g[4 + e] = acc[3][j][e];
-        swap16(v[e], v[4 + e]);
-        swap16(g[e], g[4 + e]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] += bv[e];
-        g[e] += bg[e];
-        h[e] = v[e] * act_f(g[e], a.act);
-      }
-      if (in && m < pr.M) {
-        const int64_t o = (int64_t)m * pr.N + n;
-        El::store8((E*)pr.out + o, 0, 8, h);
-        if (a.vout) {
-          El::store8((E*)a.vout + o, 0, 8, v);
-          El::store8((E*)a.gout + o, 0, 8, g);
+          for (int e = 0; e < 8; ++e) h[e] = v[e] * act_f(g[e], a.act);
+          const int64_t o = (int64_t)m * pr.N + n;
+          El::store8((E*)pr.out + o, 0, 8, h);
+          if (a.vout) {
+            El::store8((E*)a.vout + o, 0, 8, v);
+            El::store8((E*)a.gout + o, 0, 8, g);
+          }
         }
-      }
+      });
     });
   } else if constexpr (EPI == EPI_DH) {
-    // the saved value and gate of the items ahead are in flight while one is worked on (addresses behind the ends are clamped,
-    // their results dropped)
-    constexpr int NI = 2 * J, AHEAD = J < 4 ? NI : 4;
-    typename El::raw8 rv[AHEAD], rg[AHEAD];
-    auto fetch = [&](auto k) {
-      const int m = min(mb + (k % J) * 16, pr.M - 1), n = min(nb + (k / J) * 32, pr.N - 8);
-      const int64_t o = (int64_t)m * pr.N + n;
-      El::fetch8((const E*)a.value + o, 0, 8, rv[k % AHEAD]);
-      El::fetch8((const E*)a.gate + o, 0, 8, rg[k % AHEAD]);
-    };
-    static_for<0, AHEAD>([&](auto k) { fetch(k); });
-    static_for<0, 2>([&](auto ih) {
-      constexpr int i = 2 * ih;
-      const int n = nb + i * 16;
-      const bool in = n < pr.N;
-      float sv[8] = {}, sg[8] = {};
+    // The saved value and gate of the items ahead are in flight while one is worked on (addresses behind the ends are clamped,
+    // their results dropped).
+    // Two column halves a pass, whose sums fit the registers.
+    constexpr int PASS = HALVES < 2 ? HALVES : 2, NI = PASS * J, AHEAD = NI < 4 ? NI : 4;
+    static_for<0, HALVES / PASS>([&](auto pass) {
+      typename El::raw8 rv[AHEAD], rg[AHEAD];
+      const int np = nb + pass * (PASS * 32);
+      auto fetch = [&](auto k) {
+        const int m = min(mb + (k / PASS) * 16, pr.M - 1), n = min(np + (k % PASS) * 32, pr.N - 8);
+        const int64_t o = (int64_t)m * pr.N + n;
+        El::fetch8((const E*)a.value + o, 0, 8, rv[k % AHEAD]);
+        El::fetch8((const E*)a.gate + o, 0, 8, rg[k % AHEAD]);
+      };
+      static_for<0, AHEAD>([&](auto k) { fetch(k); });
+      float sv[PASS][8] = {}, sg[PASS][8] = {};
       static_for<0, J>([&](auto j) {
-        constexpr int k = ih * J + j;
         const int m = mb + j * 16;
-        float d[8], v[8], g[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d[e] = acc[i][j][e]; d[4 + e] = acc[i + 1][j][e];
-          swap16(d[e], d[4 + e]);
-        }
-        El::open8(rv[k % AHEAD], v);
-        El::open8(rg[k % AHEAD], g);
-        if constexpr (k + AHEAD < NI) fetch(std::integral_constant<int, k + AHEAD>{});
-        const bool ok = in && m < pr.M;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float f, df;
-          act_grad(g[e], a.act, f, df);
-          g[e] = d[e] * v[e] * df;
-          v[e] = d[e] * f;
-          sv[e] += ok ? v[e] : 0.f;
-          sg[e] += ok ? g[e] : 0.f;
-        }
-        if (ok) {
-          const int64_t o = (int64_t)m * pr.N + n;
-          El::store8((E*)a.vout + o, 0, 8, v);
-          El::store8((E*)a.gout + o, 0, 8, g);
-        }
-        // column sums over the wave's rows: 16 lanes in a fixed order; per 32 rows where the launch has split tiles
-        if ((j & 1) && a.colsum && (j == J - 1 || a.splits > 1)) {
+        static_for<0, PASS>([&](auto ih) {
+          constexpr int k = PASS * j + ih;
+          const int n = np + ih * 32;
+          const bool ok = n < pr.N && m < pr.M;
+          float d[8], v[8], g[8];
+          take(std::integral_constant<int, 2 * (pass * PASS + ih)>{}, j, d);
+          El::open8(rv[k % AHEAD], v);
+          El::open8(rg[k % AHEAD], g);
+          if constexpr (k + AHEAD < NI) fetch(std::integral_constant<int, k + AHEAD>{});
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            sv[e] = row16_sum(sv[e]);
-            sg[e] = row16_sum(sg[e]);
+            float f, df;
+            act_grad(g[e], a.act, f, df);
+            g[e] = d[e] * v[e] * df;
+            v[e] = d[e] * f;
           }
-          if (c == 0 && in) {
-            const int64_t row = (int64_t)(m0 / G::BT) * 2 + wm;
-            float* p = a.colsum + (a.splits > 1 ? row * (MF / 2) + (j0 + j) / 2 : row) * 2 * pr.N + n;
-            Elem<2>::store8(p, 0, 8, sv);
-            Elem<2>::store8(p + pr.N, 0, 8, sg);
+          if (ok) {
+            const int64_t o = (int64_t)m * pr.N + n;
+            El::store8((E*)a.vout + o, 0, 8, v);
+            El::store8((E*)a.gout + o, 0, 8, g);
           }
+          if (a.colsum) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sv[e] = sg[e] = 0.f;
+            for (int e = 0; e < 8; ++e) {
+              sv[ih][e] += ok ? v[e] : 0.f;
+              sg[ih][e] += ok ? g[e] : 0.f;
+            }
+          }
+        });
+        // column sums over the wave's rows: 16 lanes in a fixed order; per 16 rows where the launch has split tiles
+        if (a.colsum && (j == J - 1 || a.splits > 1)) {
+          static_for<0, PASS>([&](auto ih) {
+            const int n = np + ih * 32;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              sv[ih][e] = row16_sum(sv[ih][e]);
+              sg[ih][e] = row16_sum(sg[ih][e]);
+            }
+            if (c == 0 && n < pr.N) {
+              const int64_t row = (int64_t)(m0 / G::BT) * G::WM + wm;
+              float* p = a.colsum + (a.splits > 1 ? row * G::MF + j0 + j : row) * 2 * pr.N + n;
+              Elem<2>::store8(p, 0, 8, sv[ih]);
+              Elem<2>::store8(p + pr.N, 0, 8, sg[ih]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sv[ih][e] = sg[ih][e] = 0.f;
+          });
         }
       });
     });
   } else {
-    static_for<0, 2>([&](auto ih) {
-      constexpr int i = 2 * ih;
-      const int n = nb + i * 16;
-      const bool in = n < pr.N;
-      float b[8] = {};
-      if (in && a.bias[0]) El::load8((const E*)a.bias[0] + n, 0, 8, b);
-      static_for<0, J>([&](auto j) {
-        const int m = mb + j * 16;
-        float d[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d[e] = acc[i][j][e]; d[4 + e] = acc[i + 1][j][e];
-          swap16(d[e], d[4 + e]);
+    static_for<0, J>([&](auto j) {
+      static_for<0, HALVES>([&](auto ih) {
+        const int m = mb + j * 16, n = nb + ih * 32;
+        float d[8], b[8];
+        take(std::integral_constant<int, 2 * ih>{}, j, d);
+        if (n < pr.N && m < pr.M) {
+          if (a.bias[0]) {
+            El::load8((const E*)a.bias[0] + n, 0, 8, b);
+            for (int e = 0; e < 8; ++e) d[e] += b[e];
+          }
+          El::store8((E*)pr.out + (int64_t)m * pr.ldo + n, 0, 8, d);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] += b[e];
-        if (in && m < pr.M) El::store8((E*)pr.out + (int64_t)m * pr.ldo + n, 0, 8, d);
       });
     });
   }
 }
 
-template <int MF, bool PC, bool QC, int EPI, bool H>
-__global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs a) {
-  typedef Geo<MF, EPI> G;
-  constexpr int NF = G::NF, BT = G::BT, WN = G::WN, OPB = G::OPB, STAGE = G::STAGE;
+template <int NF, bool PC, bool QC, int EPI, bool H>
+__global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs a) {
+  typedef Geo<NF, EPI> G;
+  constexpr int MF = G::MF, BT = G::BT, OPB = G::OPB, STAGE = G::STAGE;
   __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int wm = wave / WN, wn = wave % WN;
+  const int wm = wave / G::WN, wn = wave % G::WN;
 
   // block -> first item: the blocks of one XCD (id mod 8) take neighbouring items, so its CUs share operand tiles in their L2;
   // then every gridDim-th
@@ -360,22 +365,23 @@ __global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
 
   // ---- what is being fetched: a stream of steps that runs two ahead of the products, across items
   // EPI_UP: P is two half tiles, value rows then gate rows, staged by the first and the second half of the waves
+  constexpr int HW = G::NW / 2;
   Stager<PC, G::BN> sp;
   Stager<QC, BT> sq;
   int f_it = it0, f_s = 0, f_ns = 0, f_lo = 0;
   const char *pb[2], *qb[2];
   const int sps = (a.K + BK - 1) / BK;
   auto f_item = [&]() {
-    const Item r = item_of<MF, EPI>(a, f_it);
+    const Item r = item_of<NF, EPI>(a, f_it);
     const FfProd& pr = a.pr[r.p];
     f_s = 0;
     f_ns = r.ns;
     f_lo = r.s_lo;
-    pb[0] = EPI == EPI_UP && wave >= WN ? pr.P[1] : pr.P[0];   // (WN is half the number of waves)
+    pb[0] = EPI == EPI_UP && wave >= HW ? pr.P[1] : pr.P[0];
     pb[1] = pr.P[1];
     qb[0] = pr.Q[0];
     qb[1] = pr.Q[1];
-    sp.init(lane, (EPI == EPI_UP ? wave % WN : wave) * 4, pr.ldp, r.n0, pr.N, a.K);
+    sp.init(lane, (EPI == EPI_UP ? wave % HW : wave) * 4, pr.ldp, r.n0, pr.N, a.K);
     sq.init(lane, wave * 4, pr.ldq, r.m0, pr.M, a.K);
   };
   f_item();
@@ -403,19 +409,19 @@ __global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
   rp.init(lane);
   rq.init(lane);
   f32x4 acc[NF][MF];                                       // [n fragment][m fragment]
-  bf16x8 fp[2][NF], fq[MF];
+  bf16x8 fp[NF], fq[2][MF];
   auto read_p = [&](int i, int buf, int ks) {              // fragments of k half ks of a stage
     const int row = EPI == EPI_UP ? (i >= NF / 2 ? BT / 2 : 0) + wn * (NF * 8) + (i % (NF / 2)) * 16 : wn * (NF * 16) + i * 16;
-    fp[ks][i] = rp.read(smem + buf * STAGE, row, ks);
+    fp[i] = rp.read(smem + buf * STAGE, row, ks);
   };
-  auto read_q = [&](int j, int buf, int ks) { fq[j] = rq.read(smem + buf * STAGE + OPB, wm * (MF * 16) + j * 16, ks); };
-  auto mul = [&](auto j, int ks) {
-    static_for<0, NF>([&](auto i) { acc[i][j] = mma<H>(fp[ks][i], fq[j], acc[i][j]); });
+  auto read_q = [&](int j, int buf, int ks) { fq[ks][j] = rq.read(smem + buf * STAGE + OPB, wm * (MF * 16) + j * 16, ks); };
+  auto mul = [&](auto i, int ks) {
+    static_for<0, MF>([&](auto j) { acc[i][j] = mma<H>(fp[i], fq[ks][j], acc[i][j]); });
   };
 
-  // Main loop: two LDS stages of 64 k, a step = two halves of 32 k, a half = MF groups of NF products.  Behind group j the Q
-  // fragment it used is free and is read for the next half (P fragments alternate between two sets), so every LDS read has
-  // about MF groups to land.  Once per step, behind the first group of the second half (it covers the last reads' latency),
+  // Main loop: two LDS stages of 64 k, a step = two halves of 32 k, a half = NF groups of MF products.  Behind group i the P
+  // fragment it used is free and is read for the next half (Q fragments alternate between two sets), so every LDS read has
+  // about NF groups to land.  Once per step, behind the first group of the second half (it covers the last reads' latency),
   // the waves meet: all have the stage in registers and all pieces of the next stage are in LDS; the stage is then refilled
   // with the step after the next, whose loads have a whole step to land.  The stream does not stop at an item's end: the next
   // item's first stages land while this one's tile is written.
@@ -428,29 +434,29 @@ __global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
   asm volatile("" ::: "memory");
   int buf = 0;
   for (int it = it0; it < a.items; it += gridDim.x) {
-    const Item r = item_of<MF, EPI>(a, it);
-    static_for<0, NF>([&](auto i) { read_p(i, buf, 0); });   // (read again behind an epilogue: it needs the registers)
-    static_for<0, MF>([&](auto j) { read_q(j, buf, 0); });
+    const Item r = item_of<NF, EPI>(a, it);
+    static_for<0, MF>([&](auto j) { read_q(j, buf, 0); });   // (read again behind an epilogue: it needs the registers)
+    static_for<0, NF>([&](auto i) { read_p(i, buf, 0); });
     static_for<0, NF>([&](auto i) { static_for<0, MF>([&](auto j) { acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}; }); });
     for (int s = 0; s < r.ns; ++s) {
-      static_for<0, MF>([&](auto j) {
-        mul(j, 0);
-        read_q(j, buf, 1);
-        if constexpr (j < NF) read_p(j, buf, 1);
+      static_for<0, NF>([&](auto i) {
+        mul(i, 0);
+        read_p(i, buf, 1);
+        if constexpr (i < MF) read_q(i, buf, 1);
         __builtin_amdgcn_sched_barrier(0);
       });
       open();
-      static_for<0, MF>([&](auto j) {
-        mul(j, 1);
-        if constexpr (j == 0) {
+      static_for<0, NF>([&](auto i) {
+        mul(i, 1);
+        if constexpr (i == 0) {
           __builtin_amdgcn_sched_barrier(0);
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
         }
-        static_for<j * 8 / MF, (j + 1) * 8 / MF>([&](auto e) { piece(e, buf); });
-        read_q(j, buf ^ 1, 0);                             // (behind the very last step: zeros, not used)
-        if constexpr (j < NF) read_p(j, buf ^ 1, 0);
+        static_for<i * 8 / NF, (i + 1) * 8 / NF>([&](auto e) { piece(e, buf); });
+        read_p(i, buf ^ 1, 0);                             // (behind the very last step: zeros, not used)
+        if constexpr (i < MF) read_q(i, buf ^ 1, 0);
         __builtin_amdgcn_sched_barrier(0);
       });
       buf ^= 1;
@@ -459,32 +465,29 @@ __global__ __launch_bounds__(MF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
       f32x4* p = (f32x4*)a.part + (((int64_t)r.slot * G::NW + wave) * (NF * MF)) * 64 + lane;
       static_for<0, NF>([&](auto i) { static_for<0, MF>([&](auto j) { p[(i * MF + j) * 64] = acc[i][j]; }); });
     } else {
-      epilogue<MF, EPI, H, MF>(a, a.pr[r.p], acc, r.m0, r.n0, wm, wn, 0);
+      epilogue<NF, EPI, H, MF>(a, a.pr[r.p], acc, r.m0, r.n0, wm, wn, 0);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no piece outlives the kernel
 }
 
-// adds a split tile's partials in split order and writes it; a block takes two m fragments of each wave's tile
-template <int MF, int EPI, bool H>
-__global__ __launch_bounds__(MF == 8 ? 512 : 256) void ff_finish_kernel(FfArgs a) {
-  typedef Geo<MF, EPI> G;
-  constexpr int NF = G::NF;
+// adds a split tile's partials in split order and writes it; a block takes one m fragment of each wave's tile
+template <int NF, int EPI, bool H>
+__global__ __launch_bounds__(NF == 8 ? 512 : 256) void ff_finish_kernel(FfArgs a) {
+  typedef Geo<NF, EPI> G;
+  constexpr int MF = G::MF;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int tile = blockIdx.x / (MF / 2), j0 = blockIdx.x % (MF / 2) * 2;
-  const Item r = item_of<MF, EPI>(a, a.full + tile * a.splits);
-  f32x4 acc[NF][2];
-  static_for<0, NF>([&](auto i) { acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f}; });
+  const int tile = blockIdx.x / MF, j0 = blockIdx.x % MF;
+  const Item r = item_of<NF, EPI>(a, a.full + tile * a.splits);
+  f32x4 acc[NF][1];
+  static_for<0, NF>([&](auto i) { acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; });
   const f32x4* p = (const f32x4*)a.part + (((int64_t)tile * a.splits * G::NW + wave) * (NF * MF) + j0) * 64 + lane;
 #pragma unroll 2
   for (int z = 0; z < a.splits; ++z) {
-    static_for<0, NF>([&](auto i) {
-      acc[i][0] += p[i * MF * 64];
-      acc[i][1] += p[(i * MF + 1) * 64];
-    });
+    static_for<0, NF>([&](auto i) { acc[i][0] += p[i * MF * 64]; });
     p += (int64_t)G::NW * (NF * MF) * 64;
   }
-  epilogue<MF, EPI, H, 2>(a, a.pr[r.p], acc, r.m0, r.n0, wave / G::WN, wave % G::WN, j0);
+  epilogue<NF, EPI, H, 1>(a, a.pr[r.p], acc, r.m0, r.n0, wave / G::WN, wave % G::WN, j0);
 }
 
 // column sums of [M][N] (first stage; colsum.h adds the partial rows): a wave takes 512 columns of every gridDim.y-th row
@@ -506,14 +509,14 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
 // 1.13 us (16384 x 5120 x 1280 and 512 x 20480 x 4096, bf16).  Whole rounds of tiles run as they are; the tiles of the last,
 // broken round are split along k over the idle CUs where that pays for writing and reading their float32 partials (0.117 us a
 // 256-square split tile at 4.5 TB/s over the chip, and 5 us for the second launch).
-struct Plan { int mf, full, splits, items; };
+struct Plan { int nf, full, splits, items; };
 struct Dims { int64_t M, N; };                             // output of a product; EPI_UP: N = F
 Plan pick(const Dims* d, int n, int64_t steps, int epi) {
   Plan best{};
   double least = 1e30;
-  for (int mf = 8; mf >= 4; mf -= 4) {
-    const int64_t bt = 32 * mf, bn = epi == EPI_UP ? bt / 2 : bt, slots = mf == 8 ? 256 : 512;
-    const double step = mf == 8 ? 1.5 : 1.13, part = mf == 8 ? 0.117 : 0.029;
+  for (int nf = 8; nf >= 4; nf -= 4) {
+    const int64_t bt = 32 * nf, bn = epi == EPI_UP ? bt / 2 : bt, slots = nf == 8 ? 256 : 512;
+    const double step = nf == 8 ? 1.5 : 1.13, part = nf == 8 ? 0.117 : 0.029;
     int64_t tiles = 0;
     for (int i = 0; i < n; ++i) tiles += ((d[i].M + bt - 1) / bt) * ((d[i].N + bn - 1) / bn);
     const int64_t full = tiles / slots * slots, tail = tiles - full;
@@ -521,34 +524,34 @@ Plan pick(const Dims* d, int n, int64_t steps, int epi) {
       const double us = step * steps * ((double)(full / slots) + (double)((tail * s + slots - 1) / slots) / s) + (s > 1 ? 5 + tail * s * part : 0);
       if (us < least) {
         least = us;
-        best = {mf, (int)full, (int)s, (int)(full + tail * s)};
+        best = {nf, (int)full, (int)s, (int)(full + tail * s)};
       }
       if (!tail) break;
     }
   }
   return best;
 }
-int64_t part_bytes(const Plan& p) { return p.splits > 1 ? (int64_t)(p.items - p.full) * (32 * p.mf) * (32 * p.mf) * 4 : 0; }
+int64_t part_bytes(const Plan& p) { return p.splits > 1 ? (int64_t)(p.items - p.full) * (32 * p.nf) * (32 * p.nf) * 4 : 0; }
 
-template <int MF, bool PC, bool QC, int EPI, bool H>
-void launch_mf(FfArgs& a, const Plan& p, hipStream_t st) {
-  typedef Geo<MF, EPI> G;
-  constexpr int slots = MF == 8 ? 256 : 512;
+template <int NF, bool PC, bool QC, int EPI, bool H>
+void launch_nf(FfArgs& a, const Plan& p, hipStream_t st) {
+  typedef Geo<NF, EPI> G;
+  constexpr int slots = NF == 8 ? 256 : 512;
   for (int i = 0; i < a.nprod; ++i) {
     a.pr[i].tiles_m = (a.pr[i].M + G::BT - 1) / G::BT;
     a.pr[i].tiles_n = (a.pr[i].N + G::BN - 1) / G::BN;
   }
-  hipLaunchKernelGGL((ff_gemm_kernel<MF, PC, QC, EPI, H>), dim3(p.items < slots ? p.items : slots), dim3(G::NW * 64), 0, st, a);
+  hipLaunchKernelGGL((ff_gemm_kernel<NF, PC, QC, EPI, H>), dim3(p.items < slots ? p.items : slots), dim3(G::NW * 64), 0, st, a);
   if (p.splits > 1)
-    hipLaunchKernelGGL((ff_finish_kernel<MF, EPI, H>), dim3((p.items - p.full) / p.splits * (MF / 2)), dim3(G::NW * 64), 0, st, a);
+    hipLaunchKernelGGL((ff_finish_kernel<NF, EPI, H>), dim3((p.items - p.full) / p.splits * G::MF), dim3(G::NW * 64), 0, st, a);
 }
 template <bool PC, bool QC, int EPI, bool H>
 void launch(FfArgs& a, const Plan& p, hipStream_t st) {
   a.full = p.full;
   a.splits = p.splits;
   a.items = p.items;
-  if (p.mf == 8) launch_mf<8, PC, QC, EPI, H>(a, p, st);
-  else launch_mf<4, PC, QC, EPI, H>(a, p, st);
+  if (p.nf == 8) launch_nf<8, PC, QC, EPI, H>(a, p, st);
+  else launch_nf<4, PC, QC, EPI, H>(a, p, st);
 }
 
 int64_t steps_of(int64_t k) { return (k + BK - 1) / BK; }
@@ -559,7 +562,7 @@ Plan plan_dx(int64_t M, int D, int F) { const Dims d{M, D}; return pick(&d, 1, 2
 Plan plan_dw(int64_t M, int D, int F) { const Dims d[3] = {{F, D}, {F, D}, {D, F}}; return pick(d, 3, steps_of(M), EPI_STORE); }
 Plan plan_dw2(int64_t M, int D, int F) { const Dims d[2] = {{F, D}, {F, D}}; return pick(d, 2, steps_of(M), EPI_STORE); }
 Plan plan_dw1(int64_t M, int D, int F) { const Dims d{D, F}; return pick(&d, 1, steps_of(M), EPI_STORE); }
-int64_t colsum_rows(int64_t M, const Plan& p) { return (M + 32 * p.mf - 1) / (32 * p.mf) * 2 * (p.splits > 1 ? p.mf / 2 : 1); }
+int64_t colsum_rows(int64_t M, const Plan& p) { return (M + 32 * p.nf - 1) / (32 * p.nf) * (p.nf / 2) * (p.splits > 1 ? 4 : 1); }
 constexpr int COLSUM_ROWS = 512;
 
 bool bad(int64_t M, int D, int F, int act, int dtype) {
