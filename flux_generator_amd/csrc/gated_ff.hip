@@ -463,7 +463,9 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
     }
     if (r.slot >= 0) {                                     // a partial tile, fragments as they lie in the registers
       f32x4* p = (f32x4*)a.part + (((int64_t)r.slot * G::NW + wave) * (NF * MF)) * 64 + lane;
-      static_for<0, NF>([&](auto i) { static_for<0, MF>([&](auto j) { p[(i * MF + j) * 64] = acc[i][j]; }); });
+      static_for<0, MF>([&](auto j) {                      // (rows behind the end are not looked at)
+        if (r.m0 + (wm * MF + j) * 16 < a.pr[r.p].M) static_for<0, NF>([&](auto i) { p[(i * MF + j) * 64] = acc[i][j]; });
+      });
     } else {
       epilogue<NF, EPI, H, MF>(a, a.pr[r.p], acc, r.m0, r.n0, wm, wn, 0);
     }
@@ -479,6 +481,7 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256) void ff_finish_kernel(FfArgs a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int tile = blockIdx.x / MF, j0 = blockIdx.x % MF;
   const Item r = item_of<NF, EPI>(a, a.full + tile * a.splits);
+  if (r.m0 + ((wave / G::WN) * MF + j0) * 16 >= a.pr[r.p].M && !(EPI == EPI_DH && a.colsum)) return;   // (rows behind the end: only their zero column sums)
   f32x4 acc[NF][1];
   static_for<0, NF>([&](auto i) { acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; });
   const f32x4* p = (const f32x4*)a.part + (((int64_t)tile * a.splits * G::NW + wave) * (NF * MF) + j0) * 64 + lane;
@@ -488,6 +491,80 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256) void ff_finish_kernel(FfArgs a
     p += (int64_t)G::NW * (NF * MF) * 64;
   }
   epilogue<NF, EPI, H, 1>(a, a.pr[r.p], acc, r.m0, r.n0, wave / G::WN, wave % G::WN, j0);
+}
+
+// ---- one or two tokens (serving): bound by reading the weights once.  A wave owns one output column - its value and gate row, or
+// its row of the out weight - and reads the rows whole, 1 KiB at a time and eight loads ahead, against the tokens' vectors from
+// L1; products are float32 FMAs.  4096 -> 10240 at one token: 26.8 us for 168 MB (6.3 TB/s), back 15.5 us.  (Three tokens and more: the tiles above with
+// their split along k are faster: 77 us forward at four tokens, 90 this way.)
+constexpr int GEMV = 2;
+template <bool DUAL, int MT, bool H>
+__global__ __launch_bounds__(256) void ff_gemv_kernel(FfArgs a) {
+  typedef uint16_t E;
+  typedef Elem<H ? 1 : 0> El;
+  constexpr int R = DUAL ? 2 : 1, U = 8 / R;
+  const FfProd& pr = a.pr[0];
+  const int n = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, nch = a.K / 8;
+  if (n >= pr.N) return;
+  const E *p[R], *q[MT];
+#pragma unroll
+  for (int i = 0; i < R; ++i) p[i] = (const E*)pr.P[i] + (int64_t)n * pr.ldp;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) q[m] = (const E*)pr.Q[0] + (int64_t)m * pr.ldq;
+  float acc[R][MT] = {};
+  for (int c0 = lane; c0 < nch; c0 += 64 * U) {
+    u32x4 rp[U][R], rq[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = min(c0 + u * 64, nch - 1) * 8;         // a chunk behind the end repeats the last one and becomes zeros
+#pragma unroll
+      for (int i = 0; i < R; ++i) rp[u][i] = __builtin_nontemporal_load((const u32x4*)(p[i] + c));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) rq[u][m] = *(const u32x4*)(q[m] + c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u == 0) __builtin_amdgcn_sched_barrier(0);       // (all loads before the first use)
+      const bool on = c0 + u * 64 < nch;
+#pragma unroll
+      for (int i = 0; i < R; ++i) rp[u][i] = on ? rp[u][i] : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        rq[u][m] = on ? rq[u][m] : u32x4{0, 0, 0, 0};
+        float v[8], x[8];
+        El::open8(rq[u][m], x);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          El::open8(rp[u][i], v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[i][m] = __builtin_fmaf(v[e], x[e], acc[i][m]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    float v = wave_sum(acc[0][m]), g = wave_sum(acc[R - 1][m]);
+    if (lane) continue;
+    if (a.bias[0]) v += e2f<H>(((const E*)a.bias[0])[n]);
+    const int64_t o = (int64_t)m * pr.ldo + n;
+    if constexpr (DUAL) {
+      if (a.bias[0]) g += e2f<H>(((const E*)a.bias[1])[n]);
+      if (a.vout) {
+        ((E*)a.vout)[o] = f2e<H>(v);
+        ((E*)a.gout)[o] = f2e<H>(g);
+      }
+      v *= act_f(g, a.act);
+    }
+    ((E*)pr.out)[o] = f2e<H>(v);
+  }
+}
+
+template <bool DUAL, bool H>
+void launch_gemv(const FfArgs& a, hipStream_t st) {
+  const dim3 grid((a.pr[0].N + 3) / 4);
+  if (a.pr[0].M == 1) hipLaunchKernelGGL((ff_gemv_kernel<DUAL, 1, H>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((ff_gemv_kernel<DUAL, 2, H>), grid, dim3(256), 0, st, a);
 }
 
 // column sums of [M][N] (first stage; colsum.h adds the partial rows): a wave takes 512 columns of every gridDim.y-th row
@@ -591,11 +668,14 @@ void forward(const fluxhip_gated_ff_desc* d, hipStream_t st) {
   a.nprod = a.nseg = 1; a.K = D; a.act = d->act; a.part = (float*)d->ws;
   a.vout = (char*)d->value; a.gout = (char*)d->gate;
   a.bias[0] = (const char*)d->b_value; a.bias[1] = (const char*)d->b_gate;
-  launch<false, false, EPI_UP, H>(a, plan_up(M, D, F), st);
+  a.pr[0].ldo = F;
+  if (M <= GEMV) launch_gemv<true, H>(a, st);
+  else launch<false, false, EPI_UP, H>(a, plan_up(M, D, F), st);
   FfArgs b{};
   b.pr[0] = prod(d->w_out, d->hidden, d->y, F, F, D, M, D);
   b.nprod = b.nseg = 1; b.K = F; b.part = (float*)d->ws; b.bias[0] = (const char*)d->b_out;
-  launch<false, false, EPI_STORE, H>(b, plan_down(M, D, F), st);
+  if (M <= GEMV) launch_gemv<false, H>(b, st);
+  else launch<false, false, EPI_STORE, H>(b, plan_down(M, D, F), st);
 }
 
 template <bool H>
@@ -645,7 +725,7 @@ int64_t most(int64_t a, int64_t b) { return a > b ? a : b; }
 
 extern "C" int64_t fluxhip_gated_ff_ws(int64_t M, int D, int F) {
   if (bad(M, D, F, FLUXHIP_EPI_SILU, 0)) return FLUXHIP_EINVAL;
-  return most(part_bytes(plan_up(M, D, F)), part_bytes(plan_down(M, D, F)));
+  return M <= GEMV ? 0 : most(part_bytes(plan_up(M, D, F)), part_bytes(plan_down(M, D, F)));
 }
 extern "C" int64_t fluxhip_gated_ff_grad_ws(int64_t M, int D, int F) {
   if (bad(M, D, F, FLUXHIP_EPI_SILU, 0)) return FLUXHIP_EINVAL;

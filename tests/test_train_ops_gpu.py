@@ -105,7 +105,7 @@ def test_layernorm_gradient_against_differences(dev):
 
 # ------------------------------------------------------------------------------------------------ gated feed-forward
 ACTS = {"erf": "EPI_GELU_ERF", "tanh": "EPI_GELU_TANH", "silu": "EPI_SILU"}
-FF_SHAPES = [(1, 8, 8), (1, 64, 128), (2, 128, 64), (7, 72, 200), (16, 320, 136), (17, 64, 264), (33, 640, 128), (65, 136, 72),
+FF_SHAPES = [(1, 8, 8), (1, 64, 128), (1, 1288, 5128), (2, 128, 64), (3, 520, 24), (4, 2056, 264), (5, 1032, 40), (7, 72, 200), (16, 320, 136), (17, 64, 264), (33, 640, 128), (65, 136, 72),
              (130, 128, 384), (257, 264, 520), (300, 72, 1032)]
 
 
