@@ -582,10 +582,12 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
   Elem<2>::store8(part + (int64_t)blockIdx.y * N + c, 0, 8, s);
 }
 
-// How a launch is cut.  256-square tiles run one block a CU at about 1.5 us a step (64 k) of all CUs, 128-square ones two a CU at
-// 1.13 us (16384 x 5120 x 1280 and 512 x 20480 x 4096, bf16).  Whole rounds of tiles run as they are; the tiles of the last,
-// broken round are split along k over the idle CUs where that pays for writing and reading their float32 partials (0.117 us a
-// 256-square split tile at 4.5 TB/s over the chip, and 5 us for the second launch).
+// How a launch is cut: the estimated time of every way, the least wins.  256-square tiles run one block a CU at 1.5 us a step (64 k)
+// of all CUs, 128-square ones two a CU at 1.13 us (16384 x 5120 x 1280 and 512 x 20480 x 4096, bf16).  What the epilogue moves
+// comes on top at 4.9 TB/s - all of it for the large tiles, whose CU has nothing else to run, a bit more than half for the small
+// ones (dvalue / dgate of 16384 x 2560 from 640: 130 / 112 us; of 16384 x 5120 from 1280: 329 / 345).  Whole rounds of tiles run
+// as they are; the tiles of the last, broken round are split along k over the idle CUs where that pays for writing and reading
+// their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 5 us for the second launch).
 struct Plan { int nf, full, splits, items; };
 struct Dims { int64_t M, N; };                             // output of a product; EPI_UP: N = F
 Plan pick(const Dims* d, int n, int64_t steps, int epi) {
@@ -595,10 +597,19 @@ Plan pick(const Dims* d, int n, int64_t steps, int epi) {
     const int64_t bt = 32 * nf, bn = epi == EPI_UP ? bt / 2 : bt, slots = nf == 8 ? 256 : 512;
     const double step = nf == 8 ? 1.5 : 1.13, part = nf == 8 ? 0.117 : 0.029;
     int64_t tiles = 0;
-    for (int i = 0; i < n; ++i) tiles += ((d[i].M + bt - 1) / bt) * ((d[i].N + bn - 1) / bn);
+    double out = 0, rows = 0, padded = 0;
+    for (int i = 0; i < n; ++i) {
+      const int64_t tm = (d[i].M + bt - 1) / bt;
+      tiles += tm * ((d[i].N + bn - 1) / bn);
+      out += (double)d[i].M * d[i].N;
+      rows += (double)d[i].M;
+      padded += (double)(tm * bt);
+    }
+    const double moved = out * (epi == EPI_DH ? 8 : epi == EPI_UP ? 4 : 2) / 4.9e6 * (nf == 8 ? 1.0 : 0.57);
     const int64_t full = tiles / slots * slots, tail = tiles - full;
     for (int64_t s = 1; s <= 16 && s <= steps; ++s) {
-      const double us = step * steps * ((double)(full / slots) + (double)((tail * s + slots - 1) / slots) / s) + (s > 1 ? 5 + tail * s * part : 0);
+      const double us = moved + step * steps * ((double)(full / slots) + (double)((tail * s + slots - 1) / slots) / s) +
+                        (s > 1 ? 5 + tail * s * part * (rows / padded) : 0);
       if (us < least) {
         least = us;
         best = {nf, (int)full, (int)s, (int)(full + tail * s)};
