@@ -587,7 +587,7 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
 // comes on top at 4.9 TB/s - all of it for the large tiles, whose CU has nothing else to run, a bit more than half for the small
 // ones (dvalue / dgate of 16384 x 2560 from 640: 130 / 112 us; of 16384 x 5120 from 1280: 329 / 345).  Whole rounds of tiles run
 // as they are; the tiles of the last, broken round are split along k over the idle CUs where that pays for writing and reading
-// their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 5 us for the second launch).
+// their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 8 us for the second launch).
 struct Plan { int nf, full, splits, items; };
 struct Dims { int64_t M, N; };                             // output of a product; EPI_UP: N = F
 Plan pick(const Dims* d, int n, int64_t steps, int epi) {
@@ -609,7 +609,7 @@ Plan pick(const Dims* d, int n, int64_t steps, int epi) {
     const int64_t full = tiles / slots * slots, tail = tiles - full;
     for (int64_t s = 1; s <= 16 && s <= steps; ++s) {
       const double us = moved + step * steps * ((double)(full / slots) + (double)((tail * s + slots - 1) / slots) / s) +
-                        (s > 1 ? 5 + tail * s * part * (rows / padded) : 0);
+                        (s > 1 ? 8 + tail * s * part * (rows / padded) : 0);
       if (us < least) {
         least = us;
         best = {nf, (int)full, (int)s, (int)(full + tail * s)};
@@ -702,12 +702,15 @@ void backward(const fluxhip_gated_ff_grad_desc* d, hipStream_t st) {
     a.part = (float*)((char*)d->ws + (d->db_value ? colsum_rows(M, p) * 2 * F * 4 : 0));
     a.colsum = d->db_value ? (float*)d->ws : nullptr;
     launch<true, false, EPI_DH, H>(a, p, st);
-    if (d->db_value) {
-      launch_colsum_final(a.colsum, colsum_rows(M, p), 1, 2, F, d->db_value, d->db_gate, H ? 1 : 0, st);
-      const int rows = (int)(M < COLSUM_ROWS ? M : COLSUM_ROWS);
-      hipLaunchKernelGGL((ff_colsum_kernel<H>), dim3((D + 511) / 512, rows), dim3(64), 0, st, (const uint16_t*)d->dy, d->lddy, (int)M, D,
-                         (float*)d->ws);
-      launch_colsum_final((const float*)d->ws, rows, 1, 1, D, d->db_out, nullptr, H ? 1 : 0, st);
+    if (d->db_value) {                                     // dy's columns: few rows are added up by the same launch as they are
+      Extra e{d->dy, d->db_out, d->lddy, M, D, 0};
+      if (M > 4 * COLSUM_ROWS) {
+        float* part = (float*)d->ws + colsum_rows(M, p) * 2 * F;
+        hipLaunchKernelGGL((ff_colsum_kernel<H>), dim3((D + 511) / 512, COLSUM_ROWS), dim3(64), 0, st, (const uint16_t*)d->dy, d->lddy, (int)M, D,
+                           part);
+        e = Extra{part, d->db_out, D, COLSUM_ROWS, D, 1};
+      }
+      launch_colsum_final(a.colsum, colsum_rows(M, p), 1, 2, F, d->db_value, d->db_gate, H ? 1 : 0, st, e);
     }
   }
   if (d->dx) {
@@ -741,7 +744,7 @@ extern "C" int64_t fluxhip_gated_ff_ws(int64_t M, int D, int F) {
 extern "C" int64_t fluxhip_gated_ff_grad_ws(int64_t M, int D, int F) {
   if (bad(M, D, F, FLUXHIP_EPI_SILU, 0)) return FLUXHIP_EINVAL;
   const Plan dh = plan_dh(M, D, F);
-  int64_t b = most(colsum_rows(M, dh) * 2 * F * 4 + part_bytes(dh), (int64_t)COLSUM_ROWS * D * 4);
+  int64_t b = colsum_rows(M, dh) * 2 * F * 4 + most(part_bytes(dh), (int64_t)COLSUM_ROWS * D * 4);
   b = most(b, part_bytes(plan_dx(M, D, F)));
   b = most(b, most(part_bytes(plan_dw(M, D, F)), part_bytes(plan_dw2(M, D, F))));
   return most(b, part_bytes(plan_dw1(M, D, F)));

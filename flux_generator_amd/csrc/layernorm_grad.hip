@@ -23,6 +23,7 @@ struct LnArgs {
   float *mean, *rstd, *part;
   int64_t x_bs, x_rs, dy_bs, dy_rs;   // element strides of sample / row
   int64_t T, p_bs;                    // rows per sample; elements between the samples' parameter vectors (0: shared)
+  int row_blocks, B;                  // ln_bwd_kernel without PG: blocks behind these add up parameter gradients
   int D, p_f32, direct;               // direct: one block sees every row behind a gradient vector and writes it, no partial rows
   float eps, offset;
 };
@@ -135,6 +136,37 @@ __global__ __launch_bounds__(64 * WAVES, NCH == 1 ? 8 : 4) void ln_fwd_kernel(Ln
   }
 }
 
+// dgamma (or dbeta) of 64 columns from the inputs, for few rows: eight waves take every eighth row, added in wave order
+template <int T>
+DEVINL void param_columns(const LnArgs& a, int block, int64_t sample) {
+  using E = typename Elem<T>::type;
+  __shared__ float lds[WAVES][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nc = (a.D + 63) / 64, which = block / nc, col = (block - which * nc) * 64 + lane;
+  const int c = min(col, a.D - 1);
+  float s = 0.f;
+  const int64_t b0 = a.p_bs ? sample : 0, b1 = a.p_bs ? sample + 1 : a.B;
+  for (int64_t b = b0; b < b1; ++b) {
+    const E *x = (const E*)a.x + b * a.x_bs + c, *dy = (const E*)a.dy + b * a.dy_bs + c;
+    if (which) {
+#pragma unroll 8
+      for (int64_t t = w; t < a.T; t += WAVES) s += Elem<T>::get(dy + t * a.dy_rs);
+    } else {
+#pragma unroll 8
+      for (int64_t t = w; t < a.T; t += WAVES)
+        s += Elem<T>::get(dy + t * a.dy_rs) * ((Elem<T>::get(x + t * a.x_rs) - a.mean[b * a.T + t]) * a.rstd[b * a.T + t]);
+    }
+  }
+  lds[w][lane] = s;
+  __syncthreads();
+  if (w || col >= a.D) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) s += lds[i][lane];
+  void* out = which ? a.dbeta : a.dgamma;
+  if (a.p_f32) ((float*)out)[sample * a.D + col] = s;
+  else Elem<T>::put((E*)out + sample * a.D + col, s);
+}
+
 // PG: also the parameter gradient: one partial row [2][D] per block, or the gradient itself (a.direct).
 template <int T, int WPR, int NCH, bool FULL, bool PG>
 __global__ __launch_bounds__(64 * WAVES, !PG ? (NCH == 1 ? 6 : 4) : NCH == 1 ? 4 : 2) void ln_bwd_kernel(LnArgs a) {
@@ -142,9 +174,15 @@ __global__ __launch_bounds__(64 * WAVES, !PG ? (NCH == 1 ? 6 : 4) : NCH == 1 ? 4
   constexpr int NT = 64 * WPR, RPB = WAVES / WPR;
   __shared__ float2 red[2][WAVES];
   __shared__ float comb[PG ? NCH * 8 * NT * RPB : 1];
+  if constexpr (!PG) {
+    if ((int)blockIdx.x >= a.row_blocks) {
+      if (a.p_bs || blockIdx.y == 0) param_columns<T>(a, blockIdx.x - a.row_blocks, blockIdx.y);
+      return;
+    }
+  }
   int turn = 0;
   const int tr = threadIdx.x % NT, sub = threadIdx.x / NT;
-  const int64_t b = blockIdx.y, step = (int64_t)gridDim.x * RPB;
+  const int64_t b = blockIdx.y, step = (int64_t)(PG ? gridDim.x : a.row_blocks) * RPB;
   const E *xb = (const E*)a.x + b * a.x_bs, *db_ = (const E*)a.dy + b * a.dy_bs;
   int64_t t0 = (int64_t)blockIdx.x * RPB;
   typename Elem<T>::raw8 wx[NCH], wd[NCH];
@@ -387,18 +425,26 @@ void launch_fwd(const LnArgs& a, int64_t B, hipStream_t st) {
 #undef LN_F
 }
 
+// A parameter vector that few rows feed is added up by extra blocks of the same launch, which read those rows a second time
+// (231 x 771 float32: one launch of 9 us instead of 9 + 2.5 and the second launch's 3 us on the host).
+constexpr int64_t FEW_ROWS = 512;
+
 template <int T>
 void launch_bwd(LnArgs a, int64_t B, hipStream_t st) {
-  const bool pg = a.dgamma != nullptr, shared = pg && a.p_bs == 0;
+  const bool pg = a.dgamma != nullptr, shared = pg && a.p_bs == 0, few = pg && (shared ? B * a.T : a.T) <= FEW_ROWS;
   const Shape s = pick(B * a.T, a.D, T == 2, pg);
-  const int64_t np = partials(B, a.T, a.D, s), nx = pg && s.wpr ? np : even_blocks(B, row_groups(a.T, s), 1024);
-  const dim3 grid((unsigned)nx, (unsigned)B);
-  a.direct = s.wpr && np == 1 && (B == 1 || !shared);
+  const int64_t np = partials(B, a.T, a.D, s);
+  a.direct = pg && s.wpr && np == 1 && (B == 1 || !shared);
+  const bool fold = few && s.wpr && !a.direct;
+  const int64_t nx = pg && s.wpr && !fold ? np : even_blocks(B, row_groups(a.T, s), 1024);
+  a.row_blocks = (int)nx;
+  a.B = (int)B;
+  const dim3 grid((unsigned)(nx + (fold ? (a.D + 63) / 64 * 2 : 0)), (unsigned)B);
+#define LN_B(W, N, FULL, PG) hipLaunchKernelGGL((ln_bwd_kernel<T, W, N, FULL, PG>), grid, dim3(64 * WAVES), 0, st, a)
   if (!s.wpr) {
     hipLaunchKernelGGL((ln_wide_kernel<T, true>), grid, dim3(256), 0, st, a);
     if (pg) hipLaunchKernelGGL((ln_wide_param_kernel<T>), dim3((a.D + 2047) / 2048, (unsigned)np, (unsigned)B), dim3(256), 0, st, a);
-  } else if (pg) {
-#define LN_B(W, N, FULL, PG) hipLaunchKernelGGL((ln_bwd_kernel<T, W, N, FULL, PG>), grid, dim3(64 * WAVES), 0, st, a)
+  } else if (pg && !fold) {
     if (a.D % 8 == 0) {
       LN_DISPATCH(LN_B, true, true);
     } else {
@@ -408,9 +454,9 @@ void launch_bwd(LnArgs a, int64_t B, hipStream_t st) {
     LN_DISPATCH(LN_B, true, false);
   } else {
     LN_DISPATCH(LN_B, false, false);
-#undef LN_B
   }
-  if (pg && !a.direct) {
+#undef LN_B
+  if (pg && !fold && !a.direct) {
     const int dt = a.p_f32 ? 2 : T;
     if (shared) launch_colsum_final(a.part, B * np, 1, 2, a.D, a.dgamma, a.dbeta, dt, st);
     else launch_colsum_final(a.part, np, B, 2, a.D, a.dgamma, a.dbeta, dt, st);

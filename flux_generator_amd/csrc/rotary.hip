@@ -40,13 +40,14 @@ struct Vec {
   DEVINL void put(int j, float v) { Elem<T>::put(&w[j], v); }
 };
 
-// V: elements per vector (interleaved: V / 2 pairs; half: V pairs, two vectors), dividing the rotated columns.  A thread takes
+// V: elements per vector (interleaved: V / 2 pairs; half: V pairs, two vectors), 16 bytes; the last vector of a part may be cut
+// and is then moved by element (all rows only need element alignment).  A thread takes
 // UNROLL (token, head) items at a time, all loads before the first use; the first batch's loads go out before the block works on
 // its angles.
 template <int T, int V, bool INTER, bool INV>
 __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
   using E = typename Elem<T>::type;
-  constexpr int UNROLL = V * sizeof(E) == 16 && INTER ? 4 : 2;
+  constexpr int UNROLL = INTER ? 4 : 2;
   extern __shared__ float2 cs[];       // [tb][rot / 2]
   const int np = a.rot >> 1;
   const int64_t tok0 = (int64_t)blockIdx.x * a.tb, b0 = tok0 / a.T;
@@ -54,7 +55,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
 
   const int heads = a.H + a.K, per = 256 / a.lanes;       // `lanes` threads cover a head's slots, `per` heads side by side
   const int row = threadIdx.x / a.lanes, lane = threadIdx.x - row * a.lanes;
-  const int rot_slots = INTER ? a.rot / V : np / V, step = per * gridDim.y, items = row < per ? ntb * heads : 0;
+  const int part = INTER ? a.rot : np, rot_slots = (part + V - 1) / V, step = per * gridDim.y, items = row < per ? ntb * heads : 0;
   const int first = row + blockIdx.y * per;
 
   const E* x[UNROLL];
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
       const int64_t hh = isk ? h - a.H : h;
       x[u] = (const E*)r.x + b * r.xb + t * r.xt + hh * r.xh;
       y[u] = (E*)r.y + b * r.yb + t * r.yt + hh * r.yh;
-      if (slot < rot_slots) {
+      if ((slot + 1) * V <= part) {
         p[u].load(x[u] + slot * V);
         if constexpr (!INTER) q[u].load(x[u] + np + slot * V);
       }
@@ -115,6 +116,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
           } else {
             for (int e = c; e < a.hd; ++e) y[u][e] = x[u][e];
           }
+        } else if ((slot + 1) * V > part) {               // the cut vector
+          for (int e = slot * V; e < part; e += INTER ? 2 : 1) {
+            const float2 c = w[INTER ? e >> 1 : e];
+            const int f = INTER ? e + 1 : np + e;
+            const float m = Elem<T>::get(x[u] + e), n = Elem<T>::get(x[u] + f);
+            Elem<T>::put(y[u] + e, m * c.x - n * c.y);
+            Elem<T>::put(y[u] + f, m * c.y + n * c.x);
+          }
         } else if constexpr (INTER) {
           Vec<T, V> o;
 #pragma unroll
@@ -142,13 +151,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
   }
 }
 
-template <int T, int V>
-void launch_v(const RopeArgs& a, int interleaved, int inverse, dim3 grid, size_t lds, hipStream_t st) {
+template <int T>
+void launch(const RopeArgs& a, int interleaved, int inverse, dim3 grid, size_t lds, hipStream_t st) {
+  constexpr int V = T == 2 ? 4 : 8;
   if (interleaved) {
-    if constexpr (V >= 2) {
-      if (inverse) hipLaunchKernelGGL((rotary_kernel<T, V, true, true>), grid, dim3(256), lds, st, a);
-      else hipLaunchKernelGGL((rotary_kernel<T, V, true, false>), grid, dim3(256), lds, st, a);
-    }
+    if (inverse) hipLaunchKernelGGL((rotary_kernel<T, V, true, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, V, true, false>), grid, dim3(256), lds, st, a);
   } else {
     if (inverse) hipLaunchKernelGGL((rotary_kernel<T, V, false, true>), grid, dim3(256), lds, st, a);
     else hipLaunchKernelGGL((rotary_kernel<T, V, false, false>), grid, dim3(256), lds, st, a);
@@ -179,11 +187,8 @@ extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   a.pb = d->pos_strides[0]; a.pt = d->pos_strides[1]; a.pos64 = d->pos64; a.n_axes = d->n_axes;
   a.ax1 = ax[1]; a.ax2 = ax[2]; a.ax3 = ax[3];
   a.ntok = ntok; a.T = (int)d->T; a.H = d->H; a.K = d->K; a.hd = d->hd; a.rot = d->rot; a.scale = d->scale;
-  // vectors: 16 bytes where the rotated columns (halves) divide into them; the loads themselves take any address
-  const int part = d->interleaved ? d->rot : d->rot / 2, tail = d->hd - d->rot, most = d->dtype == 2 ? 4 : 8;
-  int V = most;
-  while (part % V) V >>= 1;                               // (interleaved: rot is even, so V >= 2)
-  a.slots = part / V + (tail + V - 1) / V;
+  const int part = d->interleaved ? d->rot : d->rot / 2, tail = d->hd - d->rot, V = d->dtype == 2 ? 4 : 8;
+  a.slots = (part + V - 1) / V + (tail + V - 1) / V;
   a.lanes = a.slots < 256 ? a.slots : 256;
   const int per = 256 / a.lanes, heads = d->H + d->K, np = d->rot / 2;
   a.magic = (uint32_t)(((1ull << 32) + heads - 1) / heads);
@@ -201,10 +206,8 @@ extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   const dim3 grid((unsigned)nb, (unsigned)gy);
   const size_t lds = (size_t)tb * np * sizeof(float2);
   hipStream_t st = (hipStream_t)stream;
-#define ROPE(T, V) launch_v<T, V>(a, d->interleaved, d->inverse, grid, lds, st)
-  if (d->dtype == 0) { if (V == 8) ROPE(0, 8); else if (V == 4) ROPE(0, 4); else if (V == 2) ROPE(0, 2); else ROPE(0, 1); }
-  else if (d->dtype == 1) { if (V == 8) ROPE(1, 8); else if (V == 4) ROPE(1, 4); else if (V == 2) ROPE(1, 2); else ROPE(1, 1); }
-  else { if (V == 4) ROPE(2, 4); else if (V == 2) ROPE(2, 2); else ROPE(2, 1); }
-#undef ROPE
+  if (d->dtype == 0) launch<0>(a, d->interleaved, d->inverse, grid, lds, st);
+  else if (d->dtype == 1) launch<1>(a, d->interleaved, d->inverse, grid, lds, st);
+  else launch<2>(a, d->interleaved, d->inverse, grid, lds, st);
   return hipGetLastError() == hipSuccess ? FLUXHIP_OK : FLUXHIP_ELAUNCH;
 }

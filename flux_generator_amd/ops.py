@@ -1262,11 +1262,11 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, saved, w_value: torch.T
             if t is not None:
                 t.zero_()
         return (dx, *dw, *db)
-    dvalue, dgate = _new(value), _new(value)
-    n = lib.fluxhip_gated_ff_grad_ws(M, D, F)
-    ws = x.new_empty(n, dtype=torch.uint8)
+    n, mid = lib.fluxhip_gated_ff_grad_ws(M, D, F), -(-2 * M * F // 256) * 256      # scratch: dvalue, dgate, workspace
+    scratch = x.new_empty(2 * mid + n, dtype=torch.uint8)
+    sp = scratch.data_ptr()
     d = GatedFfGradDesc(dy.data_ptr(), x.data_ptr(), value.data_ptr(), gate.data_ptr(), hidden.data_ptr(), w_value.data_ptr(), w_gate.data_ptr(),
-                        w_out.data_ptr(), dvalue.data_ptr(), dgate.data_ptr(), *[_ptr(t) for t in (dx, *dw, *db)], M, ldx, lddy, D, F, act,
-                        _DT[x.dtype], ws.data_ptr(), n)
+                        w_out.data_ptr(), sp, sp + mid, *[_ptr(t) for t in (dx, *dw, *db)], M, ldx, lddy, D, F, act,
+                        _DT[x.dtype], sp + 2 * mid, n)
     _check(lib.fluxhip_gated_ff_grad(d, st), "fluxhip_gated_ff_grad")
     return (dx, *dw, *db)
