@@ -3,8 +3,8 @@
 //   forward   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) r, y = xh g + b          g = offset + gamma
 //   backward  e = dy g, dx = r (e - mean(e) - xh mean(e xh)), dgamma = sum_rows dy xh, dbeta = sum_rows dy
 //
-// Both are HBM-bound: a row is read once into registers (8-element chunks, chunk c of a row on thread c mod (64 WPR) of the row's
-// group, as in norm.hip), statistics are float32 and two-pass over the registers.  gamma / beta are [D], or one vector per
+// Both are HBM-bound: a row is read once into registers (8-element chunks, chunk c of a row on the c-th of its threads, modulo
+// their number), statistics are float32 and two-pass over the registers.  gamma / beta are [D], or one vector per
 // sample ([B][D], adaLN) - then the reduction of their gradient stops at the sample.  Row starts need only element alignment:
 // the 16-byte loads of this chip take any address, so an odd width costs its last chunk's element loads and nothing else.
 // The parameter gradient is a two-stage sum in a fixed order: every block adds its rows' contributions in registers and
@@ -28,10 +28,10 @@ struct LnArgs {
   float eps, offset;
 };
 
-// blocks of eight waves: 8 / WPR rows side by side, WPR waves a row
+// blocks of eight waves: a row has NT threads (16, or 1, 2, 4, 8 waves), 512 / NT rows lie side by side
 constexpr int WAVES = 8;
 
-// sums (one or two at once) over the WPR waves that share a row; red: two slots, used in turn (a slot is rewritten only behind
+// sums (one or two at once) over the NT threads that share a row; red: two slots, used in turn (a slot is rewritten only behind
 // the next barrier, which every reader of it has passed)
 DEVINL float wave_total(float v) {
   v = row16_sum(v);
@@ -39,11 +39,13 @@ DEVINL float wave_total(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16)) +
          __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 48));
 }
-template <int WPR>
+template <int NT>
 DEVINL float2 row_sum2(float a, float b, float2 (*red)[WAVES], int& turn) {
+  if constexpr (NT == 16) return make_float2(row16_sum(a), row16_sum(b));
+  constexpr int WPR = NT / 64;
   a = wave_total(a);
   b = wave_total(b);
-  if constexpr (WPR == 1) return make_float2(a, b);
+  if constexpr (NT <= 64) return make_float2(a, b);
   const int s = turn, w = threadIdx.x >> 6, w0 = w & ~(WPR - 1);
   turn ^= 1;
   if ((threadIdx.x & 63) == 0) red[s][w] = make_float2(a, b);
@@ -85,10 +87,10 @@ DEVINL void load_param(const void* p, int64_t off, int f32, int tr, int D, float
 
 // Both kernels walk rows with a stride of the grid and keep the next row's loads in flight while they reduce this one.  A row
 // group without a row left (the last round) repeats the sample's last row and drops what it computes: every wave meets every barrier.
-template <int T, int WPR, int NCH, bool FULL>
+template <int T, int NT, int NCH, bool FULL>
 __global__ __launch_bounds__(64 * WAVES, NCH == 1 ? 8 : 4) void ln_fwd_kernel(LnArgs a) {
   using E = typename Elem<T>::type;
-  constexpr int NT = 64 * WPR, RPB = WAVES / WPR;
+  constexpr int RPB = 64 * WAVES / NT;
   __shared__ float2 red[2][WAVES];
   int turn = 0;
   const int tr = threadIdx.x % NT, sub = threadIdx.x / NT;
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(64 * WAVES, NCH == 1 ? 8 : 4) void ln_fwd_kernel(Ln
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
       for (int j = 0; j < 8; ++j) s += v[i][j];           // elements behind the row's end are zeros
-    const float mu = row_sum2<WPR>(s, 0.f, red, turn).x * inv;
+    const float mu = row_sum2<NT>(s, 0.f, red, turn).x * inv;
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(64 * WAVES, NCH == 1 ? 8 : 4) void ln_fwd_kernel(Ln
         const float d = v[i][j] - mu;
         q += (tr + i * NT) * 8 + j < a.D ? d * d : 0.f;
       }
-    const float r = 1.0f / sqrtf(row_sum2<WPR>(q, 0.f, red, turn).x * inv + a.eps);
+    const float r = 1.0f / sqrtf(row_sum2<NT>(q, 0.f, red, turn).x * inv + a.eps);
     if (t < a.T) {
       const int64_t row = b * a.T + t;
       E* y = (E*)a.y + row * a.D;
@@ -168,10 +170,10 @@ DEVINL void param_columns(const LnArgs& a, int block, int64_t sample) {
 }
 
 // PG: also the parameter gradient: one partial row [2][D] per block, or the gradient itself (a.direct).
-template <int T, int WPR, int NCH, bool FULL, bool PG>
+template <int T, int NT, int NCH, bool FULL, bool PG>
 __global__ __launch_bounds__(64 * WAVES, !PG ? (NCH == 1 ? 6 : 4) : NCH == 1 ? 4 : 2) void ln_bwd_kernel(LnArgs a) {
   using E = typename Elem<T>::type;
-  constexpr int NT = 64 * WPR, RPB = WAVES / WPR;
+  constexpr int RPB = 64 * WAVES / NT;
   __shared__ float2 red[2][WAVES];
   __shared__ float comb[PG ? NCH * 8 * NT * RPB : 1];
   if constexpr (!PG) {
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(64 * WAVES, !PG ? (NCH == 1 ? 6 : 4) : NCH == 1 ? 4
       }
       if constexpr (T < 2) asm volatile("" : "+v"(cx[i]), "+v"(cd[i]));  // unpack again below: half the registers across the reduction
     }
-    const float2 s = row_sum2<WPR>(s1, s2, red, turn);
+    const float2 s = row_sum2<NT>(s1, s2, red, turn);
     if (t < a.T) {
       E* dx = (E*)a.y + (b * a.T + t) * a.D;
 #pragma unroll
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(256) void ln_wide_kernel(LnArgs a) {
           s2 += e * (v[j] - mu) * r;
         }
       }
-      const float2 t2 = row_sum2<4>(s1, s2, red, turn);
+      const float2 t2 = row_sum2<256>(s1, s2, red, turn);
       s1 = t2.x * inv;
       s2 = t2.y * inv;
     } else {
@@ -314,12 +316,12 @@ __global__ __launch_bounds__(256) void ln_wide_kernel(LnArgs a) {
         Elem<T>::load8(x, c, a.D, v);
         for (int j = 0; j < 8; ++j) s += v[j];
       }
-      mu = row_sum2<4>(s, 0.f, red, turn).x * inv;
+      mu = row_sum2<256>(s, 0.f, red, turn).x * inv;
       for (int c = threadIdx.x * 8; c < a.D; c += 2048) {
         Elem<T>::load8(x, c, a.D, v);
         for (int j = 0; j < 8; ++j) q += c + j < a.D ? (v[j] - mu) * (v[j] - mu) : 0.f;
       }
-      r = 1.0f / sqrtf(row_sum2<4>(q, 0.f, red, turn).x * inv + a.eps);
+      r = 1.0f / sqrtf(row_sum2<256>(q, 0.f, red, turn).x * inv + a.eps);
       if (threadIdx.x == 0) {
         a.mean[row] = mu;
         a.rstd[row] = r;
@@ -362,26 +364,27 @@ __global__ __launch_bounds__(256) void ln_wide_param_kernel(LnArgs a) {
   Elem<2>::store8(part + a.D, c, a.D, db);
 }
 
-// Waves per row and chunks per lane.  Few rows, float32, a parameter gradient or a width that cuts a chunk: as many waves as give
-// a lane one chunk - short serial work, and registers stay free for the loads in flight.  Else two or three chunks a lane, which
+// Threads per row and chunks per thread.  Few rows, float32, a parameter gradient or a width that cuts a chunk: as many threads as
+// have one chunk each - short serial work, and registers stay free for the loads in flight.  Else two or three chunks a lane, which
 // leaves fewer idle lanes and fewer barriers.  Measured (us, several chunks / one): 16384 x 1280 f16 forward 20.2 / 23.4, dx alone
 // 24.1 / 24.8, with parameter gradient 45.4 / 42.2; 4 x 4096 x 2560 bf16 36.4 / 40.6, 41.8 / 43.1, 59.0 / 52.9; 16384 x 1280
 // float32 32.3 / 30.1, 62.9 / 41.7, 62.8 / 55.6.
-struct Shape { int wpr, nch; };
+struct Shape { int nt, nch; };
 Shape pick(int64_t rows, int D, bool f32, bool pg) {
   const int c = (D + 7) / 8;
   const bool several = rows >= 2048 && !f32 && !pg && D % 8 == 0;
-  if (c <= 64) return {1, 1};
-  if (several && c <= 192) return {1, (c + 63) / 64};
-  if (c <= 128) return {2, 1};
-  if (c <= 256) return {4, 1};
-  if (several && c <= 384) return {4, 2};
-  if (c <= 512) return {8, 1};
-  if (c <= 1024) return {8, 2};
+  if (c <= 16) return {16, 1};
+  if (c <= 64) return {64, 1};
+  if (several && c <= 192) return {64, (c + 63) / 64};
+  if (c <= 128) return {128, 1};
+  if (c <= 256) return {256, 1};
+  if (several && c <= 384) return {256, 2};
+  if (c <= 512) return {512, 1};
+  if (c <= 1024) return {512, 2};
   return {0, 0};
 }
 int64_t row_groups(int64_t T, Shape s) {
-  const int64_t rpb = s.wpr == 0 ? 1 : WAVES / s.wpr;
+  const int64_t rpb = s.nt == 0 ? 1 : 64 * WAVES / s.nt;
   return (T + rpb - 1) / rpb;
 }
 // blocks per sample: `most` in all, every block the same number of rounds (but the last)
@@ -392,31 +395,32 @@ int64_t even_blocks(int64_t B, int64_t groups, int64_t most) {
 // partial rows per sample.  Two blocks a CU in all; at least four rounds a block, since every partial row is read again.
 int64_t partials(int64_t B, int64_t T, int D, Shape s) {
   const int64_t groups = row_groups(T, s);
-  if (groups <= 4 && s.wpr) return 1;                     // a handful of rows: one block, no second launch
-  if (!s.wpr) return groups < 64 ? groups : 64;
+  if (groups <= 4 && s.nt) return 1;                     // a handful of rows: one block, no second launch
+  if (!s.nt) return groups < 64 ? groups : 64;
   const int64_t n = even_blocks(B, groups, 512);
   return n > (groups + 3) / 4 ? (groups + 3) / 4 : n;
 }
 
 #define LN_DISPATCH(KERNEL, ...)                                              \
-  if (s.wpr == 1 && s.nch == 1) KERNEL(1, 1, __VA_ARGS__);                    \
-  else if (s.wpr == 1 && s.nch == 2) KERNEL(1, 2, __VA_ARGS__);               \
-  else if (s.wpr == 1) KERNEL(1, 3, __VA_ARGS__);                             \
-  else if (s.wpr == 2) KERNEL(2, 1, __VA_ARGS__);                             \
-  else if (s.wpr == 4 && s.nch == 1) KERNEL(4, 1, __VA_ARGS__);               \
-  else if (s.wpr == 4) KERNEL(4, 2, __VA_ARGS__);                             \
-  else if (s.nch == 1) KERNEL(8, 1, __VA_ARGS__);                             \
-  else KERNEL(8, 2, __VA_ARGS__)
+  if (s.nt == 16) KERNEL(16, 1, __VA_ARGS__);                                 \
+  else if (s.nt == 64 && s.nch == 1) KERNEL(64, 1, __VA_ARGS__);              \
+  else if (s.nt == 64 && s.nch == 2) KERNEL(64, 2, __VA_ARGS__);              \
+  else if (s.nt == 64) KERNEL(64, 3, __VA_ARGS__);                            \
+  else if (s.nt == 128) KERNEL(128, 1, __VA_ARGS__);                          \
+  else if (s.nt == 256 && s.nch == 1) KERNEL(256, 1, __VA_ARGS__);            \
+  else if (s.nt == 256) KERNEL(256, 2, __VA_ARGS__);                          \
+  else if (s.nch == 1) KERNEL(512, 1, __VA_ARGS__);                           \
+  else KERNEL(512, 2, __VA_ARGS__)
 
 template <int T>
 void launch_fwd(const LnArgs& a, int64_t B, hipStream_t st) {
   const Shape s = pick(B * a.T, a.D, T == 2, false);
   const dim3 grid((unsigned)even_blocks(B, row_groups(a.T, s), 1024), (unsigned)B);
-  if (!s.wpr) {
+  if (!s.nt) {
     hipLaunchKernelGGL((ln_wide_kernel<T, false>), grid, dim3(256), 0, st, a);
     return;
   }
-#define LN_F(W, N, FULL) hipLaunchKernelGGL((ln_fwd_kernel<T, W, N, FULL>), grid, dim3(64 * WAVES), 0, st, a)
+#define LN_F(NT, N, FULL) hipLaunchKernelGGL((ln_fwd_kernel<T, NT, N, FULL>), grid, dim3(64 * WAVES), 0, st, a)
   if (a.D % 8 == 0) {
     LN_DISPATCH(LN_F, true);
   } else {
@@ -434,14 +438,14 @@ void launch_bwd(LnArgs a, int64_t B, hipStream_t st) {
   const bool pg = a.dgamma != nullptr, shared = pg && a.p_bs == 0, few = pg && (shared ? B * a.T : a.T) <= FEW_ROWS;
   const Shape s = pick(B * a.T, a.D, T == 2, pg);
   const int64_t np = partials(B, a.T, a.D, s);
-  a.direct = pg && s.wpr && np == 1 && (B == 1 || !shared);
-  const bool fold = few && s.wpr && !a.direct;
-  const int64_t nx = pg && s.wpr && !fold ? np : even_blocks(B, row_groups(a.T, s), 1024);
+  a.direct = pg && s.nt && np == 1 && (B == 1 || !shared);
+  const bool fold = few && s.nt && !a.direct;
+  const int64_t nx = pg && s.nt && !fold ? np : even_blocks(B, row_groups(a.T, s), 1024);
   a.row_blocks = (int)nx;
   a.B = (int)B;
   const dim3 grid((unsigned)(nx + (fold ? (a.D + 63) / 64 * 2 : 0)), (unsigned)B);
-#define LN_B(W, N, FULL, PG) hipLaunchKernelGGL((ln_bwd_kernel<T, W, N, FULL, PG>), grid, dim3(64 * WAVES), 0, st, a)
-  if (!s.wpr) {
+#define LN_B(NT, N, FULL, PG) hipLaunchKernelGGL((ln_bwd_kernel<T, NT, N, FULL, PG>), grid, dim3(64 * WAVES), 0, st, a)
+  if (!s.nt) {
     hipLaunchKernelGGL((ln_wide_kernel<T, true>), grid, dim3(256), 0, st, a);
     if (pg) hipLaunchKernelGGL((ln_wide_param_kernel<T>), dim3((a.D + 2047) / 2048, (unsigned)np, (unsigned)B), dim3(256), 0, st, a);
   } else if (pg && !fold) {
@@ -471,6 +475,7 @@ bool bad_shape(int64_t B, int64_t T, int64_t D, int dtype) {
 
 extern "C" int64_t fluxhip_layernorm_grad_ws(int64_t B, int64_t T, int D) {
   if (bad_shape(B, T, D, 0)) return FLUXHIP_EINVAL;
+  if (B * T <= FEW_ROWS && pick(B * T, D, false, true).nt) return 0;     // added up without partial rows, whatever the parameters' shape
   return B * partials(B, T, D, pick(B * T, D, false, true)) * 2 * D * 4;
 }
 
@@ -497,7 +502,8 @@ extern "C" int fluxhip_layernorm_grad(const void* dy, int64_t dy_bs, int64_t dy_
   if (bad_shape(B, T, D, dtype)) return FLUXHIP_EINVAL;
   if (B == 0 || T == 0) return FLUXHIP_OK;                 // (the caller owns the zeros of an empty sum)
   if (!dy || !x || !dx || !mean || !rstd || (!dgamma) != (!dbeta)) return FLUXHIP_EINVAL;
-  if (dgamma && (!ws || ws_bytes < fluxhip_layernorm_grad_ws(B, T, D))) return FLUXHIP_EINVAL;
+  const int64_t need = dgamma ? fluxhip_layernorm_grad_ws(B, T, D) : 0;
+  if (need && (!ws || ws_bytes < need)) return FLUXHIP_EINVAL;
   LnArgs a{};
   a.x = x; a.dy = dy; a.gamma = gamma; a.y = dx; a.dgamma = dgamma; a.dbeta = dbeta;
   a.mean = (float*)mean; a.rstd = (float*)rstd; a.part = (float*)ws;

@@ -38,10 +38,25 @@ struct Vec {
   DEVINL void store(typename Elem<T>::type* p) const { __builtin_memcpy(p, w, sizeof(w)); }
   DEVINL float get(int j) const { return Elem<T>::get(&w[j]); }
   DEVINL void put(int j, float v) { Elem<T>::put(&w[j], v); }
+  // the last n < V elements, in pieces of 4, 2 and 1 (constant offsets: the vector stays in registers)
+  template <int N> DEVINL void piece(typename Elem<T>::type* p, int j) const { __builtin_memcpy(p + j, w + j, N * sizeof(w[0])); }
+  DEVINL void store_last(typename Elem<T>::type* p, int n) const {
+    if constexpr (V == 8) {
+      if (n & 4) {
+        piece<4>(p, 4);
+        if (n & 2) { piece<2>(p, 2); if (n & 1) piece<1>(p, 1); }
+        else if (n & 1) piece<1>(p, 3);
+        return;
+      }
+    }
+    if (n & 2) { piece<2>(p, V - 2); if (n & 1) piece<1>(p, V - 3); }
+    else if (n & 1) piece<1>(p, V - 1);
+  }
 };
 
-// V: elements per vector (interleaved: V / 2 pairs; half: V pairs, two vectors), 16 bytes; the last vector of a part may be cut
-// and is then moved by element (all rows only need element alignment).  A thread takes
+// V: elements per vector (interleaved: V / 2 pairs; half: V pairs, two vectors), 16 bytes.  Where the rotated
+// columns do not divide, the last vector is moved back to end with them and stores only what the one before it does not (in place,
+// a column still has one writer); rows only need element alignment.  A thread takes
 // UNROLL (token, head) items at a time, all loads before the first use; the first batch's loads go out before the block works on
 // its angles.
 template <int T, int V, bool INTER, bool INV>
@@ -77,9 +92,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
       const int64_t hh = isk ? h - a.H : h;
       x[u] = (const E*)r.x + b * r.xb + t * r.xt + hh * r.xh;
       y[u] = (E*)r.y + b * r.yb + t * r.yt + hh * r.yh;
-      if ((slot + 1) * V <= part) {
-        p[u].load(x[u] + slot * V);
-        if constexpr (!INTER) q[u].load(x[u] + np + slot * V);
+      if (slot < rot_slots && part >= V) {
+        const int c = min(slot * V, part - V);
+        p[u].load(x[u] + c);
+        if constexpr (!INTER) q[u].load(x[u] + np + c);
       }
     }
   };
@@ -116,35 +132,41 @@ __global__ __launch_bounds__(256) void rotary_kernel(RopeArgs a) {
           } else {
             for (int e = c; e < a.hd; ++e) y[u][e] = x[u][e];
           }
-        } else if ((slot + 1) * V > part) {               // the cut vector
-          for (int e = slot * V; e < part; e += INTER ? 2 : 1) {
+        } else if (part < V) {                            // a few columns only: by element
+          for (int e = 0; e < part; e += INTER ? 2 : 1) {
             const float2 c = w[INTER ? e >> 1 : e];
             const int f = INTER ? e + 1 : np + e;
             const float m = Elem<T>::get(x[u] + e), n = Elem<T>::get(x[u] + f);
             Elem<T>::put(y[u] + e, m * c.x - n * c.y);
             Elem<T>::put(y[u] + f, m * c.y + n * c.x);
           }
-        } else if constexpr (INTER) {
-          Vec<T, V> o;
-#pragma unroll
-          for (int j = 0; j < V / 2; ++j) {
-            const float2 c = w[slot * (V / 2) + j];
-            const float m = p[u].get(2 * j), n = p[u].get(2 * j + 1);
-            o.put(2 * j, m * c.x - n * c.y);
-            o.put(2 * j + 1, m * c.y + n * c.x);
-          }
-          o.store(y[u] + slot * V);
         } else {
+          const int c0 = min(slot * V, part - V), cnt = part - slot * V;   // cnt < V: of the last, moved vector
           Vec<T, V> o1, o2;
+          if constexpr (INTER) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float2 c = w[slot * V + j];
-            const float m = p[u].get(j), n = q[u].get(j);
-            o1.put(j, m * c.x - n * c.y);
-            o2.put(j, m * c.y + n * c.x);
+            for (int j = 0; j < V / 2; ++j) {
+              const float2 c = w[(c0 >> 1) + j];
+              const float m = p[u].get(2 * j), n = p[u].get(2 * j + 1);
+              o1.put(2 * j, m * c.x - n * c.y);
+              o1.put(2 * j + 1, m * c.y + n * c.x);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float2 c = w[c0 + j];
+              const float m = p[u].get(j), n = q[u].get(j);
+              o1.put(j, m * c.x - n * c.y);
+              o2.put(j, m * c.y + n * c.x);
+            }
           }
-          o1.store(y[u] + slot * V);
-          o2.store(y[u] + np + slot * V);
+          if (cnt >= V) {
+            o1.store(y[u] + c0);
+            if constexpr (!INTER) o2.store(y[u] + np + c0);
+          } else {
+            o1.store_last(y[u] + c0, cnt);
+            if constexpr (!INTER) o2.store_last(y[u] + np + c0, cnt);
+          }
         }
       }
     }

@@ -103,9 +103,9 @@ def test_entry_points_refuse_bad_descriptors():
     assert lib.fluxhip_layernorm_stats(16, 0, 8, None, None, 0, 0, 0.0, 16, 16, 16, 1, 1, 8, 1e-5, 3, None) == -1   # type
     assert lib.fluxhip_layernorm_stats(16, 0, 8, None, 16, 0, 0, 0.0, 16, 16, 16, 1, 1, 8, 1e-5, 0, None) == -1     # beta alone
     assert lib.fluxhip_layernorm_stats(None, 0, 8, None, None, 0, 0, 0.0, None, None, None, 0, 1, 8, 1e-5, 0, None) == 0
-    assert lib.fluxhip_layernorm_grad(16, 0, 8, 16, 0, 8, 16, 16, 16, 0, 0, 0.0, 16, 16, 16, 1, 100, 8, 0, None, 0, None) == -1   # no scratch
+    assert lib.fluxhip_layernorm_grad(16, 0, 8, 16, 0, 8, 16, 16, 16, 0, 0, 0.0, 16, 16, 16, 1, 9000, 8, 0, None, 0, None) == -1   # no scratch
     assert lib.fluxhip_layernorm_grad(16, 0, 8, 16, 0, 8, 16, 16, 16, 0, 0, 0.0, 16, 16, None, 1, 100, 8, 0, 16, 1 << 20, None) == -1
-    assert lib.fluxhip_layernorm_grad_ws(1, 100, 0) == -1 and lib.fluxhip_layernorm_grad_ws(1, 100, 8) > 0
+    assert lib.fluxhip_layernorm_grad_ws(1, 100, 0) == -1 and lib.fluxhip_layernorm_grad_ws(1, 9000, 8) > 0 and lib.fluxhip_layernorm_grad_ws(1, 100, 8) == 0
     d = _lib.RotaryDesc()
     assert lib.fluxhip_rotary(None, None) == -1 and lib.fluxhip_rotary(ctypes.byref(d), None) == -1
     d.B, d.T, d.H, d.hd, d.rot, d.n_axes = 1, 1, 1, 8, 8, 1

@@ -22,7 +22,7 @@ def D64(t):
 
 
 # ------------------------------------------------------------------------------------------------ LayerNorm
-LN_SHAPES = [(1, 1, 1), (1, 1, 8), (2, 3, 7), (1, 5, 64), (3, 77, 771), (1, 2050, 513), (2, 9, 1280), (1, 2300, 1280), (1, 2049, 1999),
+LN_SHAPES = [(1, 1, 1), (1, 1, 8), (2, 3, 7), (1, 5, 64), (2, 700, 19), (1, 3000, 128), (5, 33, 72), (3, 77, 771), (1, 2050, 513), (2, 9, 1280), (1, 2300, 1280), (1, 2049, 1999),
              (1, 6, 2560), (3, 170, 320), (2, 300, 72), (1, 513, 136), (1, 3, 4097), (2, 2, 8192), (1, 3, 8193), (1, 70, 9001)]
 
 
@@ -215,7 +215,9 @@ def test_gated_ff_gradient_against_differences(dev):
 @pytest.mark.parametrize("inter", [True, False])
 @pytest.mark.parametrize("B,T,H,K,hd,dims,far", [(1, 1, 1, 1, 2, [2], 0), (2, 3, 5, 1, 128, [128], 3_000_017), (1, 9, 24, 24, 128, [16, 56, 56], 0),
                                                  (2, 17, 10, 2, 84, [40], 900_001), (1, 5, 3, 3, 85, [42], 12), (3, 1, 32, 8, 64, [64], 2 ** 31 + 5),
-                                                 (1, 1300, 2, 1, 96, [6, 10, 2, 4], 77), (3, 40, 4, 4, 142, [142], 7), (2, 7, 3, 1, 38, [10], 0), (1, 30, 2, 2, 51, [30], 9), (1, 2, 1, 2, 1030, [1030], 5), (8, 1, 24, 8, 128, [128], 9)])
+                                                 (1, 1300, 2, 1, 96, [6, 10, 2, 4], 77), (3, 40, 4, 4, 142, [142], 7), (2, 7, 3, 1, 38, [10], 0), (1, 30, 2, 2, 51, [30], 9), (2, 11, 3, 3, 48, [12, 16, 16], 5), (1, 9, 2, 1, 70, [4, 2], 3),
+                                                 (1, 2, 1, 2, 1030, [1030], 5), (8, 1, 24, 8, 128, [128], 9)]
+                         + [(1, 5, 3, 1, 2 * n + 3, [2 * n], 1) for n in range(9, 16)])
 def test_rotary_forward_backward(dev, B, T, H, K, hd, dims, far, inter, dt):
     from flux_generator_amd import ops
     q, k = rnd(B, T, H, hd, seed=1, dt=dt), rnd(B, T, K, hd, seed=2, dt=dt)
@@ -252,6 +254,12 @@ def test_rotary_layouts(dev):
     values = qkv[..., (H + K) * hd:].clone()
     ops.rotary(q, k, pos, freqs, interleaved=False, out=(q, k))
     assert torch.equal(q, rq) and torch.equal(k, rk) and torch.equal(qkv[..., (H + K) * hd:], values)
+    for rot, inter in ((30, True), (30, False), (26, False), (44, False), (10, True)):
+        f, _ = ops.rotary_frequencies(rot, device=dev)
+        a, b = (rnd(B, T, n, hd, seed=n).to(dev) for n in (H, K))
+        want = ops.rotary(a, b, pos, f, interleaved=inter)
+        ops.rotary(a, b, pos, f, interleaved=inter, out=(a, b))
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1]), (rot, inter)
     e = ops.rotary(q[:, :0], k[:, :0], pos[:0], freqs)
     assert e[0].shape == (B, 0, H, hd) and e[1].shape == (B, 0, K, hd)
 
