@@ -50,9 +50,10 @@ DEVINL int col_f(int k) { return (k & 3) | ((k >> 1) & 4); }
 
 // 16 bytes a lane from the buffer straight into LDS at dst + 16 lane (dst wave-uniform; m0 carries it).  Inline asm because the
 // compiler, which cannot tell the two stages apart, would wait for all of these before every transposing LDS read; it has no
-// output register, and the main loop's own vmcnt waits cover it.
+// output register, and the main loop's own vmcnt waits cover it.  (s_nop: no resource register may be younger than five wait states
+// if a vector instruction wrote it, which the compiler does not look after inside inline asm.)
 DEVINL void dma16(u32x4 rs, uint32_t voff, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(voff), "s"(rs) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(voff), "s"(rs) : "memory", "m0");
 }
 
 template <bool COL, int BI>     // BI: indices of the tile, 64 (half a "row" tile), 128 or 256

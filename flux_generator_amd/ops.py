@@ -980,14 +980,17 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _samples(t: torch.Tensor, name: str, per_sample: bool):
     """(B, T, sample stride, row stride) of a [..., D] tensor with a contiguous last dimension; per_sample: B is its first dimension."""
-    if t.dim() < 1 or t.shape[-1] < 1 or (t.stride(-1) != 1 and t.shape[-1] != 1):
-        raise FluxHipError(f"{name} must be [..., D] with a contiguous last dimension")
-    shape, st, D = t.shape, t.stride(), t.shape[-1]
-    if t.is_contiguous():
+    shape = t.shape
+    D = shape[-1] if shape else 0
+    if D >= 1 and t.is_contiguous():
         rows = t.numel() // D
         if not per_sample:
             return 1, rows, 0, D
-        return shape[0], rows // max(1, shape[0]), rows // max(1, shape[0]) * D, D
+        rows //= max(1, shape[0])
+        return shape[0], rows, rows * D, D
+    st = t.stride()
+    if D < 1 or (st[-1] != 1 and D != 1):
+        raise FluxHipError(f"{name} must be [..., D] with a contiguous last dimension")
     lo = 1 if per_sample else 0                      # rows = dims lo .. -2 as one run, or (without per_sample) dims 1 .. -2 and dim 0 apart
     run = [i for i in range(t.dim() - 1) if i >= lo and shape[i] != 1]
     if not per_sample and len(run) > 1 and any(st[a] != st[b] * shape[b] for a, b in zip(run, run[1:])):
@@ -1000,10 +1003,10 @@ def _samples(t: torch.Tensor, name: str, per_sample: bool):
     return (shape[0] if lo else 1), T, (st[0] if lo else 0), (st[run[-1]] if run else D)
 
 
-def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, name: str):
+def _norm_param(p: torch.Tensor, x: torch.Tensor, name: str):
     """(per sample?, float32?) of a LayerNorm parameter: [D] or [B, D], x's type or float32."""
-    if p is None:
-        return None
+    if x.dim() < 1:
+        raise FluxHipError("x must be [..., D] with a contiguous last dimension")
     D = x.shape[-1]
     if p.dtype not in (x.dtype, F32) or not p.is_contiguous():
         raise FluxHipError(f"{name} must be a contiguous tensor of x's type or float32")
@@ -1019,10 +1022,9 @@ def _norm_args(x, gamma, beta, other=None):
         raise FluxHipError("x must be bfloat16, float16 or float32")
     if gamma is None and beta is not None:
         raise FluxHipError("beta needs gamma")
-    g, b = _norm_param(gamma, x, "gamma"), _norm_param(beta, x, "beta")
-    if g is not None and b is not None and (g != b or gamma.dtype != beta.dtype):
-        raise FluxHipError("gamma and beta must have one shape and one type")
-    per, pf = g if g is not None else (False, False)
+    per, pf = (False, False) if gamma is None else _norm_param(gamma, x, "gamma")
+    if beta is not None and (beta.shape != gamma.shape or beta.dtype != gamma.dtype or not beta.is_contiguous()):
+        raise FluxHipError("gamma and beta must be contiguous tensors of one shape and one type")
     if per and x.shape[0] > 65535:
         raise FluxHipError("per-sample parameters: at most 65535 samples")
     xs = _samples(x, "x", per)
@@ -1032,8 +1034,8 @@ def _norm_args(x, gamma, beta, other=None):
         os_ = _samples(other, "dy", per)
         if os_[:2] != xs[:2]:                        # one is a view of separate samples, the other one run of rows
             B = x.shape[0]
-            split = lambda s, t: s if s[0] == B and B > 1 else (B, s[1] // B, s[1] // B * s[3], s[3])
-            xs, os_ = split(xs, x), split(os_, other)
+            split = lambda s: s if s[0] == B and B > 1 else (B, s[1] // B, s[1] // B * s[3], s[3])
+            xs, os_ = split(xs), split(os_)
         return per, pf, xs, os_
     if xs[0] > 65535:
         raise FluxHipError("x: at most 65535 separately strided samples")
@@ -1157,6 +1159,8 @@ def _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, inverse, out):
     if k is not None:
         ko, ks, kos = place(k, outs[1], "k")
         K, kp, kop = k.shape[2], k.data_ptr(), ko.data_ptr()
+    if out is not None and kop == qo.data_ptr() and qo.numel() and ko.numel():
+        raise FluxHipError("out must give q and k memory of their own")
     st = _launch_stream((q, "q"), (k, "k"), (positions, "positions"), (freqs, "freqs"), (qo, "out"), (ko, "out"))
     d = RotaryDesc(q.data_ptr(), kp, qo.data_ptr(), kop, qs, ks, qos, kos, positions.data_ptr(), freqs.data_ptr(), (pb, pt), B, T, H, K, hd, rot,
                    interleaved, inverse, positions.dtype == torch.int64, na, tuple([w // 2 for w in dims]), _DT[q.dtype], scale)

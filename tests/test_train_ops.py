@@ -63,6 +63,7 @@ def test_rotary_refusals():
     refuses(ops.rotary, q.transpose(2, 3).contiguous().transpose(2, 3), k, p, f, match="contiguous last dimension")
     refuses(ops.rotary, q, k, p, f, out=q, match="out must give")
     refuses(ops.rotary, q, k, p, f, out=(q, z(2, 3, 4, 8)), match="out must have")
+    refuses(ops.rotary, q, q, p, f, out=(q, q), match="memory of their own")
     refuses(ops.rotary, q, k, p, f, out=(z(1, 3, 4, 8).expand(2, 3, 4, 8), k), match="broadcast")
     refuses(ops.rotary_backward, q, k, p, f, match="device tensors")
 
