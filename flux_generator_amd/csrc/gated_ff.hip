@@ -56,9 +56,8 @@ DEVINL void dma16(u32x4 rs, uint32_t voff, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(voff), "s"(rs) : "memory", "m0");
 }
 
-template <bool COL, int BI>     // BI: indices of the tile, 64 (half a "row" tile), 128 or 256
+template <bool COL, int BI, int NP>     // BI: indices of the tile (col: 128 or 256), NP: 1 KiB pieces per wave
 struct Stager {
-  static constexpr int NP = 4;                             // 1 KiB pieces per wave
   int64_t ld;
   int i0, ni, K;
   uint32_t voff[NP];
@@ -74,7 +73,7 @@ struct Stager {
       if constexpr (!COL) {
         const int row = piece * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
         voff[j] = (uint32_t)(row * ld * 2 + c * 16);
-        chunk[j & 1] = c;                                  // piece0 is even
+        chunk[j & 1] = c;                                  // (the swizzle alternates with the piece)
       } else {
         constexpr int KR = 512 / BI;                       // k rows per piece
         const int k = piece * KR + lane / (BI / 8), s = lane % (BI / 8);
@@ -178,13 +177,13 @@ DEVINL void swap16(float& a, float& b) {
   b = __uint_as_float(r[1]);
 }
 
-// A wave's tile is NF n by MF m fragments of 16 (128 or 64 columns - long pieces of output rows - by 64 rows), the block's 2 x WM
-// waves; block tile BT squared, 4 pieces of 1 KiB of either operand per wave and stage.  NF = 8: 256 square, eight waves (two a
-// SIMD); NF = 4: 128 square, four waves, two blocks a CU.
+// A wave's tile is NF n by MF m fragments of 16 (128, 96 or 64 columns - long pieces of output rows - by 64 rows), the block's
+// WN x WM waves; block tile BM x BP, of which every wave stages PP and QP pieces of 1 KiB a step.  NF = 8 and 6: 256 rows by 256 or
+// 192 columns, eight waves (two a SIMD), one block a CU; NF = 4: 128 square, four waves, two blocks a CU.
 template <int NF, int EPI>
 struct Geo {
-  static constexpr int MF = 4, BT = 32 * NF, WN = 2, WM = BT / 64, NW = WN * WM, BN = EPI == EPI_UP ? BT / 2 : BT, OPB = BT * BK * 2,
-                       STAGE = 2 * OPB;
+  static constexpr int MF = 4, BP = 32 * NF, BM = NF == 4 ? 128 : 256, WN = 2, WM = BM / 64, NW = WN * WM, BN = EPI == EPI_UP ? BP / 2 : BP;
+  static constexpr int PP = BP / 8 / NW, QP = BM / 8 / NW, OPB = BP * BK * 2, STAGE = OPB + BM * BK * 2;
 };
 
 struct Item { int p, m0, n0, s_lo, ns, slot; };            // slot: of the partial tile, -1 for a whole one
@@ -212,7 +211,7 @@ DEVINL Item item_of(const FfArgs& a, int it) {
   // bands of four row tiles: neighbouring items share operand tiles
   const int tm = a.pr[r.p].tiles_m, tn = a.pr[r.p].tiles_n, band = t / (4 * tn), bm = min(4, tm - band * 4);
   t -= band * 4 * tn;
-  r.m0 = (band * 4 + t % bm) * G::BT;
+  r.m0 = (band * 4 + t % bm) * G::BM;
   r.n0 = t / bm * G::BN;
   return r;
 }
@@ -223,9 +222,9 @@ DEVINL Item item_of(const FfArgs& a, int it) {
 template <int NF, int EPI, bool H, int J>
 DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int m0, int n0, int wm, int wn, int j0) {
   typedef Geo<NF, EPI> G;
-  constexpr int HALVES = EPI == EPI_UP ? NF / 4 : NF / 2;  // pairs of fragments = 32 columns
+  constexpr int HALVES = EPI == EPI_UP ? NF / 4 : NF / 2;  // pairs of fragments = 32 columns (EPI_UP with NF = 6: and a single one)
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int nb = n0 + wn * (HALVES * 32) + (q & 1) * 16 + (q >> 1) * 8;    // the lane's 8 columns behind the swap
+  const int nb = n0 + wn * (EPI == EPI_UP ? NF * 8 : NF * 16) + (q & 1) * 16 + (q >> 1) * 8;    // the lane's 8 columns behind the swap
   const int mb = m0 + wm * (G::MF * 16) + j0 * 16 + c;
   typedef uint16_t E;
   typedef Elem<H ? 1 : 0> El;
@@ -238,30 +237,49 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
     }
   };
   if constexpr (EPI == EPI_UP) {
+    auto put = [&](int m, int n, float (&v)[8], float (&g)[8]) {
+      float h[8];
+      if (n < pr.N && m < pr.M) {
+        if (a.bias[0]) {
+          El::load8((const E*)a.bias[0] + n, 0, 8, h);
+          for (int e = 0; e < 8; ++e) v[e] += h[e];
+          El::load8((const E*)a.bias[1] + n, 0, 8, h);
+          for (int e = 0; e < 8; ++e) g[e] += h[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = v[e] * act_f(g[e], a.act);
+        const int64_t o = (int64_t)m * pr.N + n;
+        El::store8((E*)pr.out + o, 0, 8, h);
+        if (a.vout) {
+          El::store8((E*)a.vout + o, 0, 8, v);
+          El::store8((E*)a.gout + o, 0, 8, g);
+        }
+      }
+    };
     static_for<0, J>([&](auto j) {
       static_for<0, HALVES>([&](auto ih) {
-        const int m = mb + j * 16, n = nb + ih * 32;
-        float v[8], g[8], h[8];
+        float v[8], g[8];
         take(std::integral_constant<int, 2 * ih>{}, j, v);
         take(std::integral_constant<int, 2 * ih + NF / 2>{}, j, g);
-        if (n < pr.N && m < pr.M) {
-          if (a.bias[0]) {
-            El::load8((const E*)a.bias[0] + n, 0, 8, h);
-            for (int e = 0; e < 8; ++e) v[e] += h[e];
-            El::load8((const E*)a.bias[1] + n, 0, 8, h);
-            for (int e = 0; e < 8; ++e) g[e] += h[e];
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = v[e] * act_f(g[e], a.act);
-          const int64_t o = (int64_t)m * pr.N + n;
-          El::store8((E*)pr.out + o, 0, 8, h);
-          if (a.vout) {
-            El::store8((E*)a.vout + o, 0, 8, v);
-            El::store8((E*)a.gout + o, 0, 8, g);
-          }
-        }
+        put(mb + j * 16, nb + ih * 32, v, g);
       });
     });
+    if constexpr (NF / 2 % 2) {                            // the odd fragment pairs with itself 16 rows on: 8 columns of either row
+      static_assert(J % 2 == 0, "two row fragments at a time");
+      constexpr int i = NF / 2 - 1;
+      static_for<0, J / 2>([&](auto jh) {
+        constexpr int j = 2 * jh;
+        float v[8], g[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[i][j][e]; v[4 + e] = acc[i][j + 1][e];
+          g[e] = acc[i + NF / 2][j][e]; g[4 + e] = acc[i + NF / 2][j + 1][e];
+          swap16(v[e], v[4 + e]);
+          swap16(g[e], g[4 + e]);
+        }
+        put(mb + (j + (q & 1)) * 16, nb - (q & 1) * 16 + i * 16, v, g);
+      });
+    }
   } else if constexpr (EPI == EPI_DH) {
     // The saved value and gate of the items ahead are in flight while one is worked on (addresses behind the ends are clamped,
     // their results dropped).
@@ -319,7 +337,7 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
               sg[ih][e] = row16_sum(sg[ih][e]);
             }
             if (c == 0 && n < pr.N) {
-              const int64_t row = (int64_t)(m0 / G::BT) * G::WM + wm;
+              const int64_t row = (int64_t)(m0 / G::BM) * G::WM + wm;
               float* p = a.colsum + (a.splits > 1 ? row * G::MF + j0 + j : row) * 2 * pr.N + n;
               Elem<2>::store8(p, 0, 8, sv[ih]);
               Elem<2>::store8(p + pr.N, 0, 8, sg[ih]);
@@ -349,9 +367,10 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
 }
 
 template <int NF, bool PC, bool QC, int EPI, bool H>
-__global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs a) {
+__global__ __launch_bounds__(NF == 4 ? 256 : 512, 2) void ff_gemm_kernel(FfArgs a) {
   typedef Geo<NF, EPI> G;
-  constexpr int MF = G::MF, BT = G::BT, OPB = G::OPB, STAGE = G::STAGE;
+  constexpr int MF = G::MF, OPB = G::OPB, STAGE = G::STAGE, PT = G::PP + G::QP;
+  static_assert(!PC || NF != 6, "a col tile's swizzle wants 128 or 256 columns");
   __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / G::WN, wn = wave % G::WN;
@@ -367,8 +386,8 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
   // ---- what is being fetched: a stream of steps that runs two ahead of the products, across items
   // EPI_UP: P is two half tiles, value rows then gate rows, staged by the first and the second half of the waves
   constexpr int HW = G::NW / 2;
-  Stager<PC, G::BN> sp;
-  Stager<QC, BT> sq;
+  Stager<PC, G::BN, G::PP> sp;
+  Stager<QC, G::BM, G::QP> sq;
   int f_it = it0, f_s = 0, f_ns = 0, f_lo = 0;
   const char *pb[2], *qb[2];
   const int sps = (a.K + BK - 1) / BK;
@@ -382,8 +401,8 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
     pb[1] = pr.P[1];
     qb[0] = pr.Q[0];
     qb[1] = pr.Q[1];
-    sp.init(lane, (EPI == EPI_UP ? wave % HW : wave) * 4, pr.ldp, r.n0, pr.N, a.K);
-    sq.init(lane, wave * 4, pr.ldq, r.m0, pr.M, a.K);
+    sp.init(lane, (EPI == EPI_UP ? wave % HW : wave) * G::PP, pr.ldp, r.n0, pr.N, a.K);
+    sq.init(lane, wave * G::QP, pr.ldq, r.m0, pr.M, a.K);
   };
   f_item();
   auto open = [&]() {                                      // resources of the stream's next step
@@ -397,22 +416,22 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
     sq.step(seg ? qb[1] : qb[0], k0, on);
     f_s += on ? 1 : 0;
   };
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 4096;
-  auto piece = [&](int j, int buf) {                       // j-th of the wave's 8 pieces of a stage
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  auto piece = [&](int j, int buf) {                       // j-th of the wave's pieces of a stage
     const uint32_t d = lds0 + buf * STAGE;
-    if (j < 4) sp.piece(j, d);
-    else sq.piece(j - 4, d + OPB);
+    if (j < G::PP) sp.piece(j, d + wave * (G::PP * 1024));
+    else sq.piece(j - G::PP, d + OPB + wave * (G::QP * 1024));
   };
 
   // ---- products
-  Reader<PC, BT> rp;
-  Reader<QC, BT> rq;
+  Reader<PC, G::BP> rp;
+  Reader<QC, G::BM> rq;
   rp.init(lane);
   rq.init(lane);
   f32x4 acc[NF][MF];                                       // [n fragment][m fragment]
   bf16x8 fp[NF], fq[2][MF];
   auto read_p = [&](int i, int buf, int ks) {              // fragments of k half ks of a stage
-    const int row = EPI == EPI_UP ? (i >= NF / 2 ? BT / 2 : 0) + wn * (NF * 8) + (i % (NF / 2)) * 16 : wn * (NF * 16) + i * 16;
+    const int row = EPI == EPI_UP ? (i >= NF / 2 ? G::BP / 2 : 0) + wn * (NF * 8) + (i % (NF / 2)) * 16 : wn * (NF * 16) + i * 16;
     fp[i] = rp.read(smem + buf * STAGE, row, ks);
   };
   auto read_q = [&](int j, int buf, int ks) { fq[ks][j] = rq.read(smem + buf * STAGE + OPB, wm * (MF * 16) + j * 16, ks); };
@@ -427,10 +446,10 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
   // with the step after the next, whose loads have a whole step to land.  The stream does not stop at an item's end: the next
   // item's first stages land while this one's tile is written.
   open();
-  static_for<0, 8>([&](auto j) { piece(j, 0); });
+  static_for<0, PT>([&](auto j) { piece(j, 0); });
   open();
-  static_for<0, 8>([&](auto j) { piece(j, 1); });
-  asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  static_for<0, PT>([&](auto j) { piece(j, 1); });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PT) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   int buf = 0;
@@ -455,7 +474,7 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
         }
-        static_for<i * 8 / NF, (i + 1) * 8 / NF>([&](auto e) { piece(e, buf); });
+        static_for<i * PT / NF, (i + 1) * PT / NF>([&](auto e) { piece(e, buf); });
         read_p(i, buf ^ 1, 0);                             // (behind the very last step: zeros, not used)
         if constexpr (i < MF) read_q(i, buf ^ 1, 0);
         __builtin_amdgcn_sched_barrier(0);
@@ -476,7 +495,7 @@ __global__ __launch_bounds__(NF == 8 ? 512 : 256, 2) void ff_gemm_kernel(FfArgs 
 
 // adds a split tile's partials in split order and writes it; a block takes one m fragment of each wave's tile
 template <int NF, int EPI, bool H>
-__global__ __launch_bounds__(NF == 8 ? 512 : 256) void ff_finish_kernel(FfArgs a) {
+__global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a) {
   typedef Geo<NF, EPI> G;
   constexpr int MF = G::MF;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -589,26 +608,29 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
 // ones (dvalue / dgate of 16384 x 2560 from 640: 130 / 112 us; of 16384 x 5120 from 1280: 329 / 345).  Whole rounds of tiles run
 // as they are; the tiles of the last, broken round are split along k over the idle CUs where that pays for writing and reading
 // their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 8 us for the second launch).
+// 256 x 192 tiles (row operands only; 1.2 us) where they fill the CUs better: EPI_UP of 512 x 10240 is 214 of them, or 160 squares.
 struct Plan { int nf, full, splits, items; };
 struct Dims { int64_t M, N; };                             // output of a product; EPI_UP: N = F
-Plan pick(const Dims* d, int n, int64_t steps, int epi) {
+int64_t tile_rows(int nf) { return nf == 4 ? 128 : 256; }
+Plan pick(const Dims* d, int n, int64_t steps, int epi, bool rows_only = false) {
   Plan best{};
   double least = 1e30;
-  for (int nf = 8; nf >= 4; nf -= 4) {
-    const int64_t bt = 32 * nf, bn = epi == EPI_UP ? bt / 2 : bt, slots = nf == 8 ? 256 : 512;
-    const double step = nf == 8 ? 1.5 : 1.13, part = nf == 8 ? 0.117 : 0.029;
+  for (int nf = 8; nf >= 4; nf -= 2) {
+    if (nf == 6 && !rows_only) continue;
+    const int64_t bm = tile_rows(nf), bn = epi == EPI_UP ? 16 * nf : 32 * nf, slots = nf == 4 ? 512 : 256;
+    const double step = nf == 8 ? 1.5 : nf == 6 ? 1.2 : 1.13, part = 0.117 / 65536 * bm * 32 * nf;
     int64_t tiles = 0;
     double out = 0, rows = 0, padded = 0;
     for (int i = 0; i < n; ++i) {
-      const int64_t tm = (d[i].M + bt - 1) / bt;
+      const int64_t tm = (d[i].M + bm - 1) / bm;
       tiles += tm * ((d[i].N + bn - 1) / bn);
       out += (double)d[i].M * d[i].N;
       rows += (double)d[i].M;
-      padded += (double)(tm * bt);
+      padded += (double)(tm * bm);
     }
-    const double moved = out * (epi == EPI_DH ? 8 : epi == EPI_UP ? 4 : 2) / 4.9e6 * (nf == 8 ? 1.0 : 0.57);
-    const int64_t full = tiles / slots * slots, tail = tiles - full;
-    for (int64_t s = 1; s <= 16 && s <= steps; ++s) {
+    const double moved = out * (epi == EPI_DH ? 8 : epi == EPI_UP ? 4 : 2) / 4.9e6 * (nf == 4 ? 0.57 : 1.0);
+    const int64_t full = tiles / slots * slots, tail = tiles - full, most = nf == 6 && epi == EPI_UP ? 1 : 16;
+    for (int64_t s = 1; s <= most && s <= steps; ++s) {
       const double us = moved + step * steps * ((double)(full / slots) + (double)((tail * s + slots - 1) / slots) / s) +
                         (s > 1 ? 8 + tail * s * part * (rows / padded) : 0);
       if (us < least) {
@@ -620,19 +642,20 @@ Plan pick(const Dims* d, int n, int64_t steps, int epi) {
   }
   return best;
 }
-int64_t part_bytes(const Plan& p) { return p.splits > 1 ? (int64_t)(p.items - p.full) * (32 * p.nf) * (32 * p.nf) * 4 : 0; }
+int64_t part_bytes(const Plan& p) { return p.splits > 1 ? (int64_t)(p.items - p.full) * tile_rows(p.nf) * (32 * p.nf) * 4 : 0; }
 
 template <int NF, bool PC, bool QC, int EPI, bool H>
 void launch_nf(FfArgs& a, const Plan& p, hipStream_t st) {
   typedef Geo<NF, EPI> G;
-  constexpr int slots = NF == 8 ? 256 : 512;
+  constexpr int slots = NF == 4 ? 512 : 256;
   for (int i = 0; i < a.nprod; ++i) {
-    a.pr[i].tiles_m = (a.pr[i].M + G::BT - 1) / G::BT;
+    a.pr[i].tiles_m = (a.pr[i].M + G::BM - 1) / G::BM;
     a.pr[i].tiles_n = (a.pr[i].N + G::BN - 1) / G::BN;
   }
   hipLaunchKernelGGL((ff_gemm_kernel<NF, PC, QC, EPI, H>), dim3(p.items < slots ? p.items : slots), dim3(G::NW * 64), 0, st, a);
-  if (p.splits > 1)
-    hipLaunchKernelGGL((ff_finish_kernel<NF, EPI, H>), dim3((p.items - p.full) / p.splits * G::MF), dim3(G::NW * 64), 0, st, a);
+  if constexpr (!(NF == 6 && EPI == EPI_UP))
+    if (p.splits > 1)
+      hipLaunchKernelGGL((ff_finish_kernel<NF, EPI, H>), dim3((p.items - p.full) / p.splits * G::MF), dim3(G::NW * 64), 0, st, a);
 }
 template <bool PC, bool QC, int EPI, bool H>
 void launch(FfArgs& a, const Plan& p, hipStream_t st) {
@@ -640,18 +663,19 @@ void launch(FfArgs& a, const Plan& p, hipStream_t st) {
   a.splits = p.splits;
   a.items = p.items;
   if (p.nf == 8) launch_nf<8, PC, QC, EPI, H>(a, p, st);
-  else launch_nf<4, PC, QC, EPI, H>(a, p, st);
+  else if (p.nf == 4) launch_nf<4, PC, QC, EPI, H>(a, p, st);
+  else if constexpr (!PC) launch_nf<6, PC, QC, EPI, H>(a, p, st);
 }
 
 int64_t steps_of(int64_t k) { return (k + BK - 1) / BK; }
-Plan plan_up(int64_t M, int D, int F) { const Dims d{M, F}; return pick(&d, 1, steps_of(D), EPI_UP); }
-Plan plan_down(int64_t M, int D, int F) { const Dims d{M, D}; return pick(&d, 1, steps_of(F), EPI_STORE); }
+Plan plan_up(int64_t M, int D, int F) { const Dims d{M, F}; return pick(&d, 1, steps_of(D), EPI_UP, true); }
+Plan plan_down(int64_t M, int D, int F) { const Dims d{M, D}; return pick(&d, 1, steps_of(F), EPI_STORE, true); }
 Plan plan_dh(int64_t M, int D, int F) { const Dims d{M, F}; return pick(&d, 1, steps_of(D), EPI_DH); }
 Plan plan_dx(int64_t M, int D, int F) { const Dims d{M, D}; return pick(&d, 1, 2 * steps_of(F), EPI_STORE); }
 Plan plan_dw(int64_t M, int D, int F) { const Dims d[3] = {{F, D}, {F, D}, {D, F}}; return pick(d, 3, steps_of(M), EPI_STORE); }
 Plan plan_dw2(int64_t M, int D, int F) { const Dims d[2] = {{F, D}, {F, D}}; return pick(d, 2, steps_of(M), EPI_STORE); }
 Plan plan_dw1(int64_t M, int D, int F) { const Dims d{D, F}; return pick(&d, 1, steps_of(M), EPI_STORE); }
-int64_t colsum_rows(int64_t M, const Plan& p) { return (M + 32 * p.nf - 1) / (32 * p.nf) * (p.nf / 2) * (p.splits > 1 ? 4 : 1); }
+int64_t colsum_rows(int64_t M, const Plan& p) { return (M + tile_rows(p.nf) - 1) / tile_rows(p.nf) * (tile_rows(p.nf) / 64) * (p.splits > 1 ? 4 : 1); }
 constexpr int COLSUM_ROWS = 512;
 
 bool bad(int64_t M, int D, int F, int act, int dtype) {

@@ -538,8 +538,8 @@ int fluxhip_layernorm_stats(const void* x, int64_t x_bs, int64_t x_rs, const voi
                             int param_f32, float offset, void* y, float* mean, float* rstd, int64_t B, int64_t T, int D,
                             float eps, int dtype, void* stream);
 /* Its gradient: dx [B][T][D] contiguous, and (both or neither) dgamma, dbeta shaped and typed like the parameters ([D], or
- * [B][D] contiguous when p_bs != 0).  ws: fluxhip_layernorm_grad_ws bytes of scratch when the parameter gradients are asked
- * for.  An empty x (B or T zero) writes nothing. */
+ * [B][D] contiguous when p_bs != 0).  ws: fluxhip_layernorm_grad_ws bytes (0 for few rows) of scratch when the parameter
+ * gradients are asked for.  An empty x (B or T zero) writes nothing.  B <= 65535. */
 int64_t fluxhip_layernorm_grad_ws(int64_t B, int64_t T, int D);
 int fluxhip_layernorm_grad(const void* dy, int64_t dy_bs, int64_t dy_rs, const void* x, int64_t x_bs, int64_t x_rs,
                            const float* mean, const float* rstd, const void* gamma, int64_t p_bs, int param_f32, float offset,
@@ -547,7 +547,7 @@ int fluxhip_layernorm_grad(const void* dy, int64_t dy_bs, int64_t dy_rs, const v
                            int64_t ws_bytes, void* stream);
 
 /* Rotary positions on q [B][T][H][hd] and k [B][T][K][hd] (element strides of batch, token, head; the last dimension is
- * contiguous; out may be in).  Pair j < rot / 2 of a token turns by positions[.., axis(j)] * freqs[j] (formed in 64 bits) and is
+ * contiguous; out may be in, but must not overlap it otherwise).  Pair j < rot / 2 of a token turns by positions[.., axis(j)] * freqs[j] (formed in 64 bits) and is
  * scaled by `scale`; columns >= rot are copied.  interleaved: pairs (2j, 2j + 1), else (j, j + rot / 2).  Axis i owns
  * axis_pairs[i] consecutive pairs (their sum is rot / 2).  inverse: the turn by the negative angle = the gradient.
  * flux/layers.py:29-33,60-75 in general form. */
@@ -586,7 +586,7 @@ int fluxhip_gated_ff(const fluxhip_gated_ff_desc* d, void* stream);
 
 /* Its gradient from dy and the saved value, gate (and hidden, for dw_out):
  *   dh = dy Wo, dvalue = dh act(gate), dgate = dh value act'(gate)   (rounded to dtype, [M][F] each, written for the products below)
- *   dx = dvalue Wv + dgate Wg, dWv = dvalue^T x, dWg = dgate^T x, dWo = dy^T hidden, db = column sums (of the unrounded values).
+ *   dx = dvalue Wv + dgate Wg, dWv = dvalue^T x, dWg = dgate^T x, dWo = dy^T hidden, db = column sums (db_value, db_gate of the unrounded values).
  * Outputs that are NULL are not computed (dw_value and dw_gate together, the three db together).  ldx, lddy % 8 == 0. */
 typedef struct fluxhip_gated_ff_grad_desc {
   const void *dy, *x, *value, *gate, *hidden, *w_value, *w_gate, *w_out;

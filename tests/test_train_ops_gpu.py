@@ -140,7 +140,7 @@ def test_gated_ff_forward_backward(dev, M, D, F, kind, dt):
     assert own[0] is None and all(torch.equal(p, q) for p, q in zip(own[1:4], out[1:4])) and own[4] is None
 
 
-@pytest.mark.parametrize("M,D,F", [(1000, 1280, 2568), (2500, 648, 4096), (3, 4096, 10240), (513, 2048, 5128)])
+@pytest.mark.parametrize("M,D,F", [(1000, 1280, 2568), (2500, 648, 4096), (3, 4096, 10240), (513, 2048, 5128), (1300, 2048, 3080), (700, 2504, 5000)])
 def test_gated_ff_larger(dev, M, D, F):
     """The large tiles, split products and many k-steps, against a float64 evaluation on the device."""
     from flux_generator_amd import ops
