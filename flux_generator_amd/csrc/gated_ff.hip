@@ -501,7 +501,8 @@ __global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int tile = blockIdx.x / MF, j0 = blockIdx.x % MF;
   const Item r = item_of<NF, EPI>(a, a.full + tile * a.splits);
-  if (r.m0 + ((wave / G::WN) * MF + j0) * 16 >= a.pr[r.p].M && !(EPI == EPI_DH && a.colsum)) return;   // (rows behind the end: only their zero column sums)
+  // (rows behind the end: only their zero column sums)
+  if (r.m0 + ((wave / G::WN) * MF + j0) * 16 >= a.pr[r.p].M && !(EPI == EPI_DH && a.colsum)) return;
   f32x4 acc[NF][1];
   static_for<0, NF>([&](auto i) { acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; });
   const f32x4* p = (const f32x4*)a.part + (((int64_t)tile * a.splits * G::NW + wave) * (NF * MF) + j0) * 64 + lane;
@@ -515,8 +516,8 @@ __global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a
 
 // ---- one or two tokens (serving): bound by reading the weights once.  A wave owns one output column - its value and gate row, or
 // its row of the out weight - and reads the rows whole, 1 KiB at a time and eight loads ahead, against the tokens' vectors from
-// L1; products are float32 FMAs.  4096 -> 10240 at one token: 26.8 us for 168 MB (6.3 TB/s), back 15.5 us.  (Three tokens and more: the tiles above with
-// their split along k are faster: 77 us forward at four tokens, 90 this way.)
+// L1; products are float32 FMAs.  4096 -> 10240 at one token: 26.8 us for 168 MB (6.3 TB/s), back 15.5 us.  (Three tokens and
+// more: the tiles above with their split along k are faster: 77 us forward at four tokens, 90 this way.)
 constexpr int GEMV = 2;
 template <bool DUAL, int MT, bool H>
 __global__ __launch_bounds__(256) void ff_gemv_kernel(FfArgs a) {
@@ -608,7 +609,8 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
 // ones (dvalue / dgate of 16384 x 2560 from 640: 130 / 112 us; of 16384 x 5120 from 1280: 329 / 345).  Whole rounds of tiles run
 // as they are; the tiles of the last, broken round are split along k over the idle CUs where that pays for writing and reading
 // their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 8 us for the second launch).
-// 256 x 192 tiles (row operands only; 1.2 us) where they fill the CUs better: EPI_UP of 512 x 10240 is 214 of them, or 160 squares.
+// 256 x 192 tiles (row operands only; 1.2 us) where they fill the CUs better: EPI_UP of 512 x 10240 from 4096 is 214 of them in
+// 108 us, or 160 squares in 118; its product back, split, 59.6 and 9.8 adding up, with squares 51 and 15.
 struct Plan { int nf, full, splits, items; };
 struct Dims { int64_t M, N; };                             // output of a product; EPI_UP: N = F
 int64_t tile_rows(int nf) { return nf == 4 ? 128 : 256; }
@@ -664,7 +666,7 @@ void launch(FfArgs& a, const Plan& p, hipStream_t st) {
   a.items = p.items;
   if (p.nf == 8) launch_nf<8, PC, QC, EPI, H>(a, p, st);
   else if (p.nf == 4) launch_nf<4, PC, QC, EPI, H>(a, p, st);
-  else if constexpr (!PC) launch_nf<6, PC, QC, EPI, H>(a, p, st);
+  else if constexpr (!PC && !QC) launch_nf<6, PC, QC, EPI, H>(a, p, st);
 }
 
 int64_t steps_of(int64_t k) { return (k + BK - 1) / BK; }
@@ -675,7 +677,9 @@ Plan plan_dx(int64_t M, int D, int F) { const Dims d{M, D}; return pick(&d, 1, 2
 Plan plan_dw(int64_t M, int D, int F) { const Dims d[3] = {{F, D}, {F, D}, {D, F}}; return pick(d, 3, steps_of(M), EPI_STORE); }
 Plan plan_dw2(int64_t M, int D, int F) { const Dims d[2] = {{F, D}, {F, D}}; return pick(d, 2, steps_of(M), EPI_STORE); }
 Plan plan_dw1(int64_t M, int D, int F) { const Dims d{D, F}; return pick(&d, 1, steps_of(M), EPI_STORE); }
-int64_t colsum_rows(int64_t M, const Plan& p) { return (M + tile_rows(p.nf) - 1) / tile_rows(p.nf) * (tile_rows(p.nf) / 64) * (p.splits > 1 ? 4 : 1); }
+int64_t colsum_rows(int64_t M, const Plan& p) {
+  return (M + tile_rows(p.nf) - 1) / tile_rows(p.nf) * (tile_rows(p.nf) / 64) * (p.splits > 1 ? 4 : 1);
+}
 constexpr int COLSUM_ROWS = 512;
 
 bool bad(int64_t M, int D, int F, int act, int dtype) {

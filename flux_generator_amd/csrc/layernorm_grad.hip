@@ -430,12 +430,15 @@ void launch_fwd(const LnArgs& a, int64_t B, hipStream_t st) {
 }
 
 // A parameter vector that few rows feed is added up by extra blocks of the same launch, which read those rows a second time
-// (231 x 771 float32: one launch of 9 us instead of 9 + 2.5 and the second launch's 3 us on the host).
-constexpr int64_t FEW_ROWS = 512;
+// (231 x 771 float32: one launch of 9 us instead of 9 + 2.5 and the second launch's 3 us on the host).  With parameters per sample
+// this holds while the second reading comes from the caches; one launch / two, bf16: 4 x 77 x 1280 3.8 / 8.0 us, 8 x 256 x 1280
+// 10.6 / 10.9, 16 x 64 x 4096 11.1 / 17.5, 16 x 256 x 1024 12.7 / 11.1, 16 x 512 x 2048 31.9 / 25.5, 256 x 77 x 1280 68 / 52.
+constexpr int64_t FEW_ROWS = 512, FEW_ELEMENTS = 1 << 22;
 
 template <int T>
 void launch_bwd(LnArgs a, int64_t B, hipStream_t st) {
-  const bool pg = a.dgamma != nullptr, shared = pg && a.p_bs == 0, few = pg && (shared ? B * a.T : a.T) <= FEW_ROWS;
+  const bool pg = a.dgamma != nullptr, shared = pg && a.p_bs == 0;
+  const bool few = pg && (shared ? B * a.T : a.T) <= FEW_ROWS && B * a.T * a.D <= FEW_ELEMENTS;
   const Shape s = pick(B * a.T, a.D, T == 2, pg);
   const int64_t np = partials(B, a.T, a.D, s);
   a.direct = pg && s.nt && np == 1 && (B == 1 || !shared);
@@ -475,7 +478,8 @@ bool bad_shape(int64_t B, int64_t T, int64_t D, int dtype) {
 
 extern "C" int64_t fluxhip_layernorm_grad_ws(int64_t B, int64_t T, int D) {
   if (bad_shape(B, T, D, 0)) return FLUXHIP_EINVAL;
-  if (B * T <= FEW_ROWS && pick(B * T, D, false, true).nt) return 0;     // added up without partial rows, whatever the parameters' shape
+  // few rows: added up without partial rows, whatever the parameters' shape
+  if (B * T <= FEW_ROWS && B * T * D <= FEW_ELEMENTS && pick(B * T, D, false, true).nt) return 0;
   return B * partials(B, T, D, pick(B * T, D, false, true)) * 2 * D * 4;
 }
 
