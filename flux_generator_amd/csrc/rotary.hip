@@ -188,8 +188,8 @@ void launch(const RopeArgs& a, int interleaved, int inverse, dim3 grid, size_t l
 }  // namespace
 
 extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
-  if (!d || d->B < 0 || d->T < 0 || d->H < 0 || d->K < 0 || d->hd < 1 || d->hd > 4096 || d->rot < 2 || d->rot > d->hd || (d->rot & 1) ||
-      d->n_axes < 1 || d->n_axes > 4 || d->dtype < 0 || d->dtype > 2)
+  if (!d || d->B < 0 || d->B > (1ll << 32) || d->T < 0 || d->T > (1 << 30) || d->H < 0 || d->K < 0 || d->hd < 1 || d->hd > 4096 ||
+      d->rot < 2 || d->rot > d->hd || (d->rot & 1) || d->n_axes < 1 || d->n_axes > 4 || d->dtype < 0 || d->dtype > 2)
     return FLUXHIP_EINVAL;
   int pairs = 0, ax[4] = {0, 1 << 30, 1 << 30, 1 << 30};
   for (int i = 0; i < d->n_axes; ++i) {
@@ -201,7 +201,8 @@ extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   if (pairs != d->rot / 2) return FLUXHIP_EINVAL;
   const int64_t ntok = d->B * d->T;
   if (ntok == 0 || d->H + d->K == 0) return FLUXHIP_OK;
-  if (d->T > (1 << 30) || d->H > 4096 || d->K > 4096 || !d->positions || !d->freqs || (d->H && (!d->q || !d->q_out)) || (d->K && (!d->k || !d->k_out))) return FLUXHIP_EINVAL;
+  if (d->H > 4096 || d->K > 4096 || !d->positions || !d->freqs ||
+      (d->H && (!d->q || !d->q_out)) || (d->K && (!d->k || !d->k_out))) return FLUXHIP_EINVAL;
   RopeArgs a{};
   a.q = {d->q, d->q_out, d->q_strides[0], d->q_strides[1], d->q_strides[2], d->qo_strides[0], d->qo_strides[1], d->qo_strides[2]};
   a.k = {d->k, d->k_out, d->k_strides[0], d->k_strides[1], d->k_strides[2], d->ko_strides[0], d->ko_strides[1], d->ko_strides[2]};

@@ -1159,7 +1159,8 @@ def _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, inverse, out):
     if k is not None:
         ko, ks, kos = place(k, outs[1], "k")
         K, kp, kop = k.shape[2], k.data_ptr(), ko.data_ptr()
-    if out is not None and kop == qo.data_ptr() and qo.numel() and ko.numel():
+    if out is not None and k is not None and q.numel() and k.numel() and \
+            (kop == qo.data_ptr() or kop == q.data_ptr() or kp == qo.data_ptr()):
         raise FluxHipError("out must give q and k memory of their own")
     st = _launch_stream((q, "q"), (k, "k"), (positions, "positions"), (freqs, "freqs"), (qo, "out"), (ko, "out"))
     d = RotaryDesc(q.data_ptr(), kp, qo.data_ptr(), kop, qs, ks, qos, kos, positions.data_ptr(), freqs.data_ptr(), (pb, pt), B, T, H, K, hd, rot,
@@ -1171,8 +1172,8 @@ def _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, inverse, out):
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, axes_dim=None,
            interleaved: bool = True, scale: float = 1.0, out=None):
     """Rotary positions on q [B, T, H, head_dim] and k [B, T, K, head_dim] (or None) in one launch -> (q', k') (or q').  Any strides
-    with a contiguous last dimension (transposed heads, slices of a fused projection); out: tensors to write, which may be the
-    inputs themselves.  positions [T] or [B, T] integers, with axes_dim of several axes [T, axes] or [B, T, axes]; freqs, scale:
+    with a contiguous last dimension (transposed heads, slices of a fused projection); out: tensors to write, which may be q and k
+    themselves but not overlap them otherwise.  positions [T] or [B, T] integers, with axes_dim of several axes [T, axes] or [B, T, axes]; freqs, scale:
     rotary_frequencies.  The first 2 len(freqs) columns turn - pairs (2j, 2j + 1) when interleaved, else (j, j + half) -, the rest is
     copied.  Angles are formed in 64 bits."""
     return _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, False, out)
@@ -1245,15 +1246,19 @@ def gated_ff(x: torch.Tensor, w_value: torch.Tensor, w_gate: torch.Tensor, w_out
 def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, saved, w_value: torch.Tensor, w_gate: torch.Tensor, w_out: torch.Tensor,
                       act: int = EPI_GELU_ERF, input_grad: bool = True, weight_grads: bool = True, bias_grads: bool = False):
     """Gradient of `gated_ff` from its saved (value, gate, hidden): (dx, dw_value, dw_gate, dw_out, db_value, db_gate, db_out), None
-    where not asked for (weight_grads=False: adapter training on frozen weights, half the work)."""
+    where not asked for (weight_grads=False: adapter training on frozen weights, half the work; hidden may then be None)."""
     D, F = _ff_weights(x, w_value, w_gate, w_out, act)
     M, ldx = _ff_rows(x, "x", D, x.dtype)
     if dy.shape != x.shape:
         raise FluxHipError("dy must have x's shape")
     _, lddy = _ff_rows(dy, "dy", D, x.dtype)
+    if not isinstance(saved, (tuple, list)) or len(saved) != 3:
+        raise FluxHipError("saved must be the (value, gate, hidden) of gated_ff(.., save=True)")
     value, gate, hidden = saved
     for t, name in ((value, "value"), (gate, "gate"), (hidden, "hidden")):
-        if t.shape != (*x.shape[:-1], F) or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16:
+        if t is None and name == "hidden" and not weight_grads:
+            continue
+        if not isinstance(t, torch.Tensor) or t.shape != (*x.shape[:-1], F) or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16:
             raise FluxHipError(f"{name} must be the contiguous [..., {F}] tensor gated_ff saved")
     st = _launch_stream((x, "x"), (dy, "dy"), (value, "value"), (gate, "gate"), (hidden, "hidden"), (w_value, "w_value"), (w_gate, "w_gate"),
                         (w_out, "w_out"))
@@ -1269,7 +1274,7 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, saved, w_value: torch.T
     n, mid = lib.fluxhip_gated_ff_grad_ws(M, D, F), -(-2 * M * F // 256) * 256      # scratch: dvalue, dgate, workspace
     scratch = x.new_empty(2 * mid + n, dtype=torch.uint8)
     sp = scratch.data_ptr()
-    d = GatedFfGradDesc(dy.data_ptr(), x.data_ptr(), value.data_ptr(), gate.data_ptr(), hidden.data_ptr(), w_value.data_ptr(), w_gate.data_ptr(),
+    d = GatedFfGradDesc(dy.data_ptr(), x.data_ptr(), value.data_ptr(), gate.data_ptr(), _ptr(hidden), w_value.data_ptr(), w_gate.data_ptr(),
                         w_out.data_ptr(), sp, sp + mid, *[_ptr(t) for t in (dx, *dw, *db)], M, ldx, lddy, D, F, act,
                         _DT[x.dtype], sp + 2 * mid, n)
     _check(lib.fluxhip_gated_ff_grad(d, st), "fluxhip_gated_ff_grad")

@@ -64,6 +64,7 @@ def test_rotary_refusals():
     refuses(ops.rotary, q, k, p, f, out=q, match="out must give")
     refuses(ops.rotary, q, k, p, f, out=(q, z(2, 3, 4, 8)), match="out must have")
     refuses(ops.rotary, q, q, p, f, out=(q, q), match="memory of their own")
+    refuses(ops.rotary, q, z(2, 3, 4, 8), p, f, out=(z(2, 3, 4, 8), q), match="memory of their own")
     refuses(ops.rotary, q, k, p, f, out=(z(1, 3, 4, 8).expand(2, 3, 4, 8), k), match="broadcast")
     refuses(ops.rotary_backward, q, k, p, f, match="device tensors")
 
@@ -91,6 +92,9 @@ def test_gated_ff_refusals():
     refuses(ops.gated_ff_backward, z(2, 16), x, s, wv, wv, wo, match="dy must have")
     refuses(ops.gated_ff_backward, x, x, (z(3, 24), z(3, 16), z(3, 24)), wv, wv, wo, match="gate must be")
     refuses(ops.gated_ff_backward, x, x, (z(3, 24), z(3, 24), z(3, 24, dt=HF)), wv, wv, wo, match="hidden must be")
+    refuses(ops.gated_ff_backward, x, x, None, wv, wv, wo, match="saved must be")
+    refuses(ops.gated_ff_backward, x, x, (z(3, 24), z(3, 24), None), wv, wv, wo, match="hidden must be")
+    refuses(ops.gated_ff_backward, x, x, (z(3, 24), z(3, 24), None), wv, wv, wo, weight_grads=False, match="device tensors")
     refuses(ops.gated_ff_backward, x, x, s, wv, wv, wo, match="device tensors")
 
 

@@ -59,8 +59,9 @@ def test_layernorm_strided_and_repeatable(dev):
     """Slices of packed buffers (samples apart, rows apart, a single column), mixed layouts of x and dy, and the same bits twice."""
     from flux_generator_amd import ops
     B, T, D = 3, 37, 640
-    buf, dbuf = rnd(B, T + 11, D + 24, seed=5).to(dev), rnd(B, T + 3, D, seed=6).to(dev)
+    buf, dbuf = (torch.full(s, float("nan"), dtype=BF, device=dev) for s in ((B, T + 11, D + 24), (B, T + 3, D)))
     x, dy = buf[:, 11:, 8:8 + D], dbuf[:, :T]
+    x.copy_(rnd(B, T, D, seed=5)); dy.copy_(rnd(B, T, D, seed=6))
     for g in (rnd(D, mean=1, seed=7).to(dev), rnd(B, D, seed=8).to(dev)):
         b = torch.zeros_like(g)
         y, mu, r = ops.layernorm(x, g, b)
@@ -136,6 +137,8 @@ def test_gated_ff_forward_backward(dev, M, D, F, kind, dt):
         R.check(got, pair, name)
     frozen = ops.gated_ff_backward(c["dy"], c["x"], (v, a, h), c["wv"], c["wg"], c["wo"], act=act, weight_grads=False)
     assert torch.equal(frozen[0], out[0]) and all(q is None for q in frozen[1:])
+    lean = ops.gated_ff_backward(c["dy"], c["x"], (v, a, None), c["wv"], c["wg"], c["wo"], act=act, weight_grads=False, bias_grads=True)
+    assert torch.equal(lean[0], out[0]) and all(torch.equal(p, q) for p, q in zip(lean[4:], out[4:]))
     own = ops.gated_ff_backward(c["dy"], c["x"], (v, a, h), c["wv"], c["wg"], c["wo"], act=act, input_grad=False)
     assert own[0] is None and all(torch.equal(p, q) for p, q in zip(own[1:4], out[1:4])) and own[4] is None
 
@@ -166,9 +169,10 @@ def test_gated_ff_strided_empty_and_repeatable(dev):
     M, D, F = 70, 64, 136
     t, b = ff_case(M, D, F, BF, True)
     c = {k: v.to(dev) for k, v in t.items()}
-    buf, dbuf = torch.zeros(M, D + 40, dtype=BF, device=dev), torch.zeros(M, D + 8, dtype=BF, device=dev)
-    buf[:, 16:16 + D], dbuf[:, :D] = c["x"], c["dy"]
-    x, dy = buf[:, 16:16 + D], dbuf[:, :D]
+    nan = float("nan")                                    # what lies around the operands is not looked at
+    buf, dbuf = torch.full((M + 9, D + 40), nan, dtype=BF, device=dev), torch.full((M + 9, D + 8), nan, dtype=BF, device=dev)
+    buf[2:2 + M, 16:16 + D], dbuf[3:3 + M, :D] = c["x"], c["dy"]
+    x, dy = buf[2:2 + M, 16:16 + D], dbuf[3:3 + M, :D]
     W = (c["wv"], c["wg"], c["wo"])
     y, s = ops.gated_ff(x, *W, save=True)
     y2, s2 = ops.gated_ff(c["x"], *W, save=True)
@@ -262,6 +266,46 @@ def test_rotary_layouts(dev):
         assert torch.equal(a, want[0]) and torch.equal(b, want[1]), (rot, inter)
     e = ops.rotary(q[:, :0], k[:, :0], pos[:0], freqs)
     assert e[0].shape == (B, 0, H, hd) and e[1].shape == (B, 0, K, hd)
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Tensors of more than 2^32 bytes and 2^31 elements: the last rows are those of a call on them alone."""
+    from flux_generator_amd import ops
+    T, H, hd = 70_000, 256, 128                            # 2.3e9 elements
+    q = torch.zeros(1, T, H, hd, dtype=BF, device=dev)
+    q[:, -3:] = rnd(1, 3, H, hd, seed=1).to(dev)
+    freqs, _ = ops.rotary_frequencies(hd, device=dev)
+    pos = torch.arange(T, device=dev) + 2 ** 33
+    assert torch.equal(ops.rotary(q, None, pos, freqs)[:, -3:], ops.rotary(q[:, -3:], None, pos[-3:], freqs))
+    D = 4096
+    x = q.view(-1, D)                                       # 560 000 rows
+    g = rnd(D, mean=1.0, seed=2).to(dev)
+    y, mu, r = ops.layernorm(x, g, g)
+    tail = ops.layernorm(x[-192:].repeat(20, 1), g, g)      # (3840 rows: the same kernel)
+    assert torch.equal(y[-192:], tail[0][-192:]) and torch.equal(mu[-192:], tail[1][-192:]) and torch.equal(r[-192:], tail[2][-192:])
+    dx, dg, db = ops.layernorm_backward(y, x, mu, r, g)
+    ex, eg, eb = ops.layernorm_backward(y[-192:].repeat(20, 1), x[-192:].repeat(20, 1), tail[1], tail[2], g)
+    assert torch.equal(dx[-192:], ex[-192:])
+    del q, x, y, dx, ex
+    M, D, F = 300_000, 8, 8192                              # value, gate, hidden: 2.5e9 elements each
+    t, b = ff_case(64, D, F, BF, True, seed=3)
+    W = [t[k].to(dev) for k in ("wv", "wg", "wo")]
+    x = torch.zeros(M, D, dtype=BF, device=dev)
+    x[-64:] = t["x"].to(dev)
+    y, s = ops.gated_ff(x, *W, *(q.to(dev) for q in b), save=True)
+    y2, s2 = ops.gated_ff(t["x"].to(dev), *W, *(q.to(dev) for q in b), save=True)
+    assert all(torch.equal(p[-64:], q) for p, q in zip(s, s2))
+    # (y's product may be split differently along k: hidden is the same, the float32 sums of 8192 terms differ in order)
+    room = 2 * F * R.E32 * (D64(s2[2]).abs() @ D64(t["wo"]).abs().t() + 1) + 2 * R.u(BF) * D64(y2).abs() * 1.01
+    assert bool(((D64(y[-64:]) - D64(y2)).abs() <= room).all())
+    dy = torch.zeros_like(x)
+    dy[-64:] = t["dy"].to(dev)
+    out = ops.gated_ff_backward(dy, x, s, *W, bias_grads=True)
+    del s
+    pairs = R.ff_backward_bound(D64(t["dy"]), D64(t["x"]), *(D64(q) for q in s2), *(D64(q) for q in (t["wv"], t["wg"], t["wo"])), "erf", BF)
+    R.check(out[0][-64:], pairs[0], "dx")
+    for name, got, (ref, bound) in zip(("dw_value", "dw_gate", "dw_out", "db_value", "db_gate", "db_out"), out[1:], pairs[1:]):
+        R.check(got, (ref, bound), name)                    # (the other rows' dy is zero: they add zeros)
 
 
 # ------------------------------------------------------------------------------------------------ together, as they are used
