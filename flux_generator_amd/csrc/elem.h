@@ -48,13 +48,14 @@ struct Elem16 {
       v[2 * j + 1] = e_hi<H>(w[j]);
     }
   }
+  static DEVINL raw8 close8(const float (&v)[8]) {
+    return raw8{e_pack<H>(v[0], v[1]), e_pack<H>(v[2], v[3]), e_pack<H>(v[4], v[5]), e_pack<H>(v[6], v[7])};
+  }
   template <bool FULL = false>
   static DEVINL void store8(type* p, int c, int n, const float (&v)[8]) {
     if (FULL ? c < n : c + 8 <= n) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = e_pack<H>(v[2 * j], v[2 * j + 1]);
-      __builtin_memcpy(p + c, w, 16);
+      const raw8 w = close8(v);
+      __builtin_memcpy(p + c, &w, 16);
     } else if (!FULL && c < n) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)

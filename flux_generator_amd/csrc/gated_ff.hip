@@ -141,17 +141,19 @@ DEVINL f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
                                                      __builtin_bit_cast(__attribute__((ext_vector_type(8))) __bf16, b), c, 0, 0, 0);
 }
 
-DEVINL float act_f(float x, int act) {
-  return act == FLUXHIP_EPI_GELU_TANH ? gelu_tanh_f(x) : act == FLUXHIP_EPI_SILU ? silu_f(x) : gelu_erf_f(x);
+template <int ACT>
+DEVINL float act_f(float x) {
+  return ACT == FLUXHIP_EPI_GELU_TANH ? gelu_tanh_f(x) : ACT == FLUXHIP_EPI_SILU ? silu_f(x) : gelu_erf_f(x);
 }
 // act(x) and act'(x).  silu: p (1 + x (1 - p)), p = sigmoid x.  tanh form: p + x p (1 - p) u', p = sigmoid(2 u).
 // erf form: Phi(x) + x phi(x), Phi from the same rational erfc as gelu_erf_f with its exponential shared.
-DEVINL void act_grad(float x, int act, float& f, float& df) {
-  if (act == FLUXHIP_EPI_SILU) {
+template <int ACT>
+DEVINL void act_grad(float x, float& f, float& df) {
+  if constexpr (ACT == FLUXHIP_EPI_SILU) {
     const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
     f = x * p;
     df = p * (1.0f + x * (1.0f - p));
-  } else if (act == FLUXHIP_EPI_GELU_TANH) {
+  } else if constexpr (ACT == FLUXHIP_EPI_GELU_TANH) {
     constexpr float c0 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, c1 = c0 * 0.044715f;
     const float x2 = x * x;
     const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * __builtin_fmaf(x2, c1, c0)));
@@ -170,6 +172,14 @@ DEVINL void act_grad(float x, int act, float& f, float& df) {
     df = phi + x * e * 0.3989422804014327f;
   }
 }
+// eight at once: one branch on the activation for all of them, not one an element (first product of 10170 x 2040 from 120, all
+// three outputs: 70 -> 61 us with its second)
+template <class F>
+DEVINL void each_act(int act, F f) {
+  if (act == FLUXHIP_EPI_SILU) f(std::integral_constant<int, FLUXHIP_EPI_SILU>{});
+  else if (act == FLUXHIP_EPI_GELU_TANH) f(std::integral_constant<int, FLUXHIP_EPI_GELU_TANH>{});
+  else f(std::integral_constant<int, FLUXHIP_EPI_GELU_ERF>{});
+}
 
 DEVINL void swap16(float& a, float& b) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
@@ -185,6 +195,17 @@ struct Geo {
   static constexpr int MF = 4, BP = 32 * NF, BM = NF == 4 ? 128 : 256, WN = 2, WM = BM / 64, NW = WN * WM, BN = EPI == EPI_UP ? BP / 2 : BP;
   static constexpr int PP = BP / 8 / NW, QP = BM / 8 / NW, OPB = BP * BK * 2, STAGE = OPB + BM * BK * 2;
 };
+
+// 16 rows by 64 columns of 16-bit elements: as the fragments lie (a, b: row = lane & 15, 64 bytes of it each) <-> as they are moved
+// (a: rows 0..7, b: rows 8..15, a whole 128-byte line of each).  Lanes 8..15 of every 16 trade their a for the b of lanes 0..7.
+DEVINL void trade8(u32x4& a, u32x4& b) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int x = (int)a[e], y = (int)b[e];
+    a[e] = (uint32_t)__builtin_amdgcn_update_dpp(x, y, 0x128, 0xf, 0xc, false);      // row_ror:8
+    b[e] = (uint32_t)__builtin_amdgcn_update_dpp(y, x, 0x128, 0xf, 0x3, false);
+  }
+}
 
 struct Item { int p, m0, n0, s_lo, ns, slot; };            // slot: of the partial tile, -1 for a whole one
 template <int NF, int EPI>
@@ -218,7 +239,8 @@ DEVINL Item item_of(const FfArgs& a, int it) {
 
 // writes J m fragments of a wave's tile, from the j0-th.  Rows outside, their columns inside: one row's pieces (of one or several
 // tensors) are written together, which keeps the pages in reach of the CU's TLB (dvalue / dgate of 16384 x 5120: 372 -> 325 us
-// against the other order).
+// against the other order), and pairs of fragments are traded into whole 128-byte lines (from 128: 200 -> 163 us; a plain copy in
+// that tiling: 157 -> 140).
 template <int NF, int EPI, bool H, int J>
 DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int m0, int n0, int wm, int wn, int j0) {
   typedef Geo<NF, EPI> G;
@@ -226,6 +248,16 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int nb = n0 + wn * (EPI == EPI_UP ? NF * 8 : NF * 16) + (q & 1) * 16 + (q >> 1) * 8;    // the lane's 8 columns behind the swap
   const int mb = m0 + wm * (G::MF * 16) + j0 * 16 + c;
+  // Traded pairs move through buffer resources whose range check ends the rows; a lane behind the last column takes an offset
+  // beyond them.  Column c0: of a pair in the tile, from the wave's first; offsets stay below 2^30 (256 rows of at most 2^21 bytes).
+  const int64_t ld = pr.N;
+  const uint32_t row_bytes = (uint32_t)pr.N * 2;
+  const int nx = nb + (c >> 3) * 32;                       // traded: the lane's 8 columns; its rows: c & 7, and 8 behind that
+  const uint32_t lane_at = (uint32_t)(wm * (G::MF * 16) + j0 * 16 + (c & 7)) * row_bytes + (uint32_t)(nx - n0) * 2;
+  auto rows_of = [&](const void* t) {
+    return __builtin_amdgcn_make_buffer_rsrc((char*)t + ((int64_t)m0 * ld + n0) * 2, 0, (int)(min(pr.M - m0, G::BM) * row_bytes), 0x00020000);
+  };
+  auto at = [&](int c0, int j) { return (nx + c0 < pr.N ? lane_at + c0 * 2 : 1u << 31) + (uint32_t)(j * 16) * row_bytes; };
   typedef uint16_t E;
   typedef Elem<H ? 1 : 0> El;
   auto take = [&](auto i, auto j, float (&d)[8]) {         // fragments i, i + 1 -> 8 neighbouring n
@@ -236,18 +268,28 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
       swap16(d[e], d[4 + e]);
     }
   };
+  auto move8 = [&](__amdgpu_buffer_rsrc_t t, const u32x4 (&r)[2], int c0, int j) {        // stores a traded pair
+    const uint32_t o = at(c0, j);
+    __builtin_amdgcn_raw_buffer_store_b128(r[0], t, o, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(r[1], t, o + 8 * row_bytes, 0, 0);
+  };
   if constexpr (EPI == EPI_UP) {
+    auto finish = [&](int n, float (&v)[8], float (&g)[8], float (&h)[8]) {
+      if (a.bias[0] && n < pr.N) {
+        El::load8((const E*)a.bias[0] + n, 0, 8, h);
+        for (int e = 0; e < 8; ++e) v[e] += h[e];
+        El::load8((const E*)a.bias[1] + n, 0, 8, h);
+        for (int e = 0; e < 8; ++e) g[e] += h[e];
+      }
+      each_act(a.act, [&](auto act) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = v[e] * act_f<act>(g[e]);
+      });
+    };
     auto put = [&](int m, int n, float (&v)[8], float (&g)[8]) {
       float h[8];
+      finish(n, v, g, h);
       if (n < pr.N && m < pr.M) {
-        if (a.bias[0]) {
-          El::load8((const E*)a.bias[0] + n, 0, 8, h);
-          for (int e = 0; e < 8; ++e) v[e] += h[e];
-          El::load8((const E*)a.bias[1] + n, 0, 8, h);
-          for (int e = 0; e < 8; ++e) g[e] += h[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = v[e] * act_f(g[e], a.act);
         const int64_t o = (int64_t)m * pr.N + n;
         El::store8((E*)pr.out + o, 0, 8, h);
         if (a.vout) {
@@ -257,12 +299,31 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
       }
     };
     static_for<0, J>([&](auto j) {
-      static_for<0, HALVES>([&](auto ih) {
-        float v[8], g[8];
-        take(std::integral_constant<int, 2 * ih>{}, j, v);
-        take(std::integral_constant<int, 2 * ih + NF / 2>{}, j, g);
-        put(mb + j * 16, nb + ih * 32, v, g);
-      });
+      float v[8], g[8];
+      if constexpr (HALVES == 2) {
+        u32x4 rh[2], rv[2], rg[2];
+        static_for<0, 2>([&](auto ih) {
+          float h[8];
+          take(std::integral_constant<int, 2 * ih>{}, j, v);
+          take(std::integral_constant<int, 2 * ih + NF / 2>{}, j, g);
+          finish(nb + ih * 32, v, g, h);
+          rh[ih] = El::close8(h);
+          rv[ih] = El::close8(v);
+          rg[ih] = El::close8(g);
+        });
+        trade8(rh[0], rh[1]);
+        move8(rows_of(pr.out), rh, 0, j);
+        if (a.vout) {
+          trade8(rv[0], rv[1]);
+          move8(rows_of(a.vout), rv, 0, j);
+          trade8(rg[0], rg[1]);
+          move8(rows_of(a.gout), rg, 0, j);
+        }
+      } else {
+        take(std::integral_constant<int, 0>{}, j, v);
+        take(std::integral_constant<int, NF / 2>{}, j, g);
+        put(mb + j * 16, nb, v, g);
+      }
     });
     if constexpr (NF / 2 % 2) {                            // the odd fragment pairs with itself 16 rows on: 8 columns of either row
       static_assert(J % 2 == 0, "two row fragments at a time");
@@ -281,44 +342,48 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
       });
     }
   } else if constexpr (EPI == EPI_DH) {
-    // The saved value and gate of the items ahead are in flight while one is worked on (addresses behind the ends are clamped,
-    // their results dropped).
-    // Two column halves a pass, whose sums fit the registers.
-    constexpr int PASS = HALVES < 2 ? HALVES : 2, NI = PASS * J, AHEAD = NI < 4 ? NI : 4;
+    // The saved value and gate of the next 16 rows are in flight while these are worked on (large tiles: from the middle of the
+    // work, where registers are free - 16384 x 5120 from 1280 298 us, 314 with 94 spilled registers from its start; small ones
+    // 163 / 168 from 128).  64 columns a pass, whose sums fit the registers.
+    constexpr int PASS = 2;
+    static_assert(HALVES % PASS == 0, "whole lines");
+    const auto value = rows_of(a.value), gate = rows_of(a.gate), vout = rows_of(a.vout), gout = rows_of(a.gout);
     static_for<0, HALVES / PASS>([&](auto pass) {
-      typename El::raw8 rv[AHEAD], rg[AHEAD];
+      u32x4 rv[2][2], rg[2][2];
       const int np = nb + pass * (PASS * 32);
-      auto fetch = [&](auto k) {
-        const int m = min(mb + (k / PASS) * 16, pr.M - 1), n = min(np + (k % PASS) * 32, pr.N - 8);
-        const int64_t o = (int64_t)m * pr.N + n;
-        El::fetch8((const E*)a.value + o, 0, 8, rv[k % AHEAD]);
-        El::fetch8((const E*)a.gate + o, 0, 8, rg[k % AHEAD]);
+      auto fetch = [&](auto j) {
+        const uint32_t o = at(pass * (PASS * 32), j);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          rv[j & 1][k] = __builtin_amdgcn_raw_buffer_load_b128(value, o + k * 8 * row_bytes, 0, 0);
+          rg[j & 1][k] = __builtin_amdgcn_raw_buffer_load_b128(gate, o + k * 8 * row_bytes, 0, 0);
+        }
       };
-      static_for<0, AHEAD>([&](auto k) { fetch(k); });
+      fetch(std::integral_constant<int, 0>{});
       float sv[PASS][8] = {}, sg[PASS][8] = {};
       static_for<0, J>([&](auto j) {
         const int m = mb + j * 16;
+        u32x4 (&qv)[2] = rv[j & 1], (&qg)[2] = rg[j & 1];
+        if constexpr (NF == 4 && j + 1 < J) fetch(std::integral_constant<int, j + 1>{});
+        trade8(qv[0], qv[1]);
+        trade8(qg[0], qg[1]);
         static_for<0, PASS>([&](auto ih) {
-          constexpr int k = PASS * j + ih;
-          const int n = np + ih * 32;
-          const bool ok = n < pr.N && m < pr.M;
+          const bool ok = np + ih * 32 < pr.N && m < pr.M;
           float d[8], v[8], g[8];
           take(std::integral_constant<int, 2 * (pass * PASS + ih)>{}, j, d);
-          El::open8(rv[k % AHEAD], v);
-          El::open8(rg[k % AHEAD], g);
-          if constexpr (k + AHEAD < NI) fetch(std::integral_constant<int, k + AHEAD>{});
+          El::open8(qv[ih], v);
+          El::open8(qg[ih], g);
+          each_act(a.act, [&](auto act) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float f, df;
-            act_grad(g[e], a.act, f, df);
-            g[e] = d[e] * v[e] * df;
-            v[e] = d[e] * f;
-          }
-          if (ok) {
-            const int64_t o = (int64_t)m * pr.N + n;
-            El::store8((E*)a.vout + o, 0, 8, v);
-            El::store8((E*)a.gout + o, 0, 8, g);
-          }
+            for (int e = 0; e < 8; ++e) {
+              float f, df;
+              act_grad<act>(g[e], f, df);
+              g[e] = d[e] * v[e] * df;
+              v[e] = d[e] * f;
+            }
+          });
+          qv[ih] = El::close8(v);
+          qg[ih] = El::close8(g);
           if (a.colsum) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -327,6 +392,11 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
             }
           }
         });
+        if constexpr (NF > 4 && j + 1 < J) fetch(std::integral_constant<int, j + 1>{});
+        trade8(qv[0], qv[1]);
+        trade8(qg[0], qg[1]);
+        move8(vout, qv, pass * (PASS * 32), j);
+        move8(gout, qg, pass * (PASS * 32), j);
         // column sums over the wave's rows: 16 lanes in a fixed order; per 16 rows where the launch has split tiles
         if (a.colsum && (j == J - 1 || a.splits > 1)) {
           static_for<0, PASS>([&](auto ih) {
@@ -349,17 +419,23 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
       });
     });
   } else {
+    const auto out = rows_of(pr.out);
+    u32x4 w[2];
     static_for<0, J>([&](auto j) {
       static_for<0, HALVES>([&](auto ih) {
-        const int m = mb + j * 16, n = nb + ih * 32;
+        const int n = nb + ih * 32;
         float d[8], b[8];
         take(std::integral_constant<int, 2 * ih>{}, j, d);
-        if (n < pr.N && m < pr.M) {
-          if (a.bias[0]) {
-            El::load8((const E*)a.bias[0] + n, 0, 8, b);
-            for (int e = 0; e < 8; ++e) d[e] += b[e];
-          }
-          El::store8((E*)pr.out + (int64_t)m * pr.ldo + n, 0, 8, d);
+        if (a.bias[0] && n < pr.N) {
+          El::load8((const E*)a.bias[0] + n, 0, 8, b);
+          for (int e = 0; e < 8; ++e) d[e] += b[e];
+        }
+        w[ih & 1] = El::close8(d);
+        if constexpr (ih & 1) {
+          trade8(w[0], w[1]);
+          move8(out, w, (ih - 1) * 32, j);
+        } else if constexpr (ih + 1 == HALVES) {           // (NF = 6: an odd one)
+          if (n < pr.N && mb + j * 16 < pr.M) __builtin_memcpy((E*)pr.out + (int64_t)(mb + j * 16) * pr.N + n, &w[0], 16);
         }
       });
     });
@@ -575,7 +651,7 @@ __global__ __launch_bounds__(256) void ff_gemv_kernel(FfArgs a) {
         ((E*)a.vout)[o] = f2e<H>(v);
         ((E*)a.gout)[o] = f2e<H>(g);
       }
-      v *= act_f(g, a.act);
+      each_act(a.act, [&](auto act) { v *= act_f<act>(g); });
     }
     ((E*)pr.out)[o] = f2e<H>(v);
   }
@@ -606,7 +682,7 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
 // How a launch is cut: the estimated time of every way, the least wins.  256-square tiles run one block a CU at 1.5 us a step (64 k)
 // of all CUs, 128-square ones two a CU at 1.13 us (16384 x 5120 x 1280 and 512 x 20480 x 4096, bf16).  What the epilogue moves
 // comes on top at 4.9 TB/s - all of it for the large tiles, whose CU has nothing else to run, a bit more than half for the small
-// ones (dvalue / dgate of 16384 x 2560 from 640: 130 / 112 us; of 16384 x 5120 from 1280: 329 / 345).  Whole rounds of tiles run
+// ones (dvalue / dgate of 16384 x 5120: from 128 178 / 163 us, from 1280 298 / 341).  Whole rounds of tiles run
 // as they are; the tiles of the last, broken round are split along k over the idle CUs where that pays for writing and reading
 // their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 8 us for the second launch).
 // 256 x 192 tiles (row operands only; 1.2 us) where they fill the CUs better: EPI_UP of 512 x 10240 from 4096 is 214 of them in
