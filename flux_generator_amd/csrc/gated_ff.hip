@@ -29,7 +29,7 @@ enum { EPI_STORE = 0, EPI_UP = 1, EPI_DH = 2 };
 struct FfProd {                 // out[m][n] = sum over segments of Q[seg] P[seg]
   const char *P[2], *Q[2];
   char* out;
-  int64_t ldp, ldq, ldo;        // element strides of the rows of P, Q, out
+  int64_t ldp, ldq;             // element strides of the rows of P, Q (out: N)
   int M, N, tiles_m, tiles_n;
 };
 // One launch: up to three products of one contraction length, their tiles in one list.  The first `full` tiles are whole work
@@ -249,13 +249,12 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
   const int nb = n0 + wn * (EPI == EPI_UP ? NF * 8 : NF * 16) + (q & 1) * 16 + (q >> 1) * 8;    // the lane's 8 columns behind the swap
   const int mb = m0 + wm * (G::MF * 16) + j0 * 16 + c;
   // Traded pairs move through buffer resources whose range check ends the rows; a lane behind the last column takes an offset
-  // beyond them.  Column c0: of a pair in the tile, from the wave's first; offsets stay below 2^30 (256 rows of at most 2^21 bytes).
-  const int64_t ld = pr.N;
+  // beyond them all (256 rows of at most 2^21 bytes).  c0: the pair's first column from the wave's.
   const uint32_t row_bytes = (uint32_t)pr.N * 2;
   const int nx = nb + (c >> 3) * 32;                       // traded: the lane's 8 columns; its rows: c & 7, and 8 behind that
   const uint32_t lane_at = (uint32_t)(wm * (G::MF * 16) + j0 * 16 + (c & 7)) * row_bytes + (uint32_t)(nx - n0) * 2;
   auto rows_of = [&](const void* t) {
-    return __builtin_amdgcn_make_buffer_rsrc((char*)t + ((int64_t)m0 * ld + n0) * 2, 0, (int)(min(pr.M - m0, G::BM) * row_bytes), 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc((char*)t + ((int64_t)m0 * pr.N + n0) * 2, 0, (int)(min(pr.M - m0, G::BM) * row_bytes), 0x00020000);
   };
   auto at = [&](int c0, int j) { return (nx + c0 < pr.N ? lane_at + c0 * 2 : 1u << 31) + (uint32_t)(j * 16) * row_bytes; };
   typedef uint16_t E;
@@ -644,7 +643,7 @@ __global__ __launch_bounds__(256) void ff_gemv_kernel(FfArgs a) {
     float v = wave_sum(acc[0][m]), g = wave_sum(acc[R - 1][m]);
     if (lane) continue;
     if (a.bias[0]) v += e2f<H>(((const E*)a.bias[0])[n]);
-    const int64_t o = (int64_t)m * pr.ldo + n;
+    const int64_t o = (int64_t)m * pr.N + n;
     if constexpr (DUAL) {
       if (a.bias[0]) g += e2f<H>(((const E*)a.bias[1])[n]);
       if (a.vout) {
@@ -671,7 +670,7 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
   const int c = (blockIdx.x * 64 + threadIdx.x) * 8;
   if (c >= N) return;
   float s[8] = {}, v[8];
-#pragma unroll 8
+#pragma unroll 16
   for (int m = blockIdx.y; m < M; m += gridDim.y) {
     El::load8(x + m * ld + c, 0, 8, v);
     for (int e = 0; e < 8; ++e) s[e] += v[e];
@@ -756,7 +755,7 @@ Plan plan_dw1(int64_t M, int D, int F) { const Dims d{D, F}; return pick(&d, 1, 
 int64_t colsum_rows(int64_t M, const Plan& p) {
   return (M + tile_rows(p.nf) - 1) / tile_rows(p.nf) * (tile_rows(p.nf) / 64) * (p.splits > 1 ? 4 : 1);
 }
-constexpr int COLSUM_ROWS = 512;
+constexpr int COLSUM_ROWS = 1024;                          // (16384 x 1280, both stages: 15.1 us, with 512 17.4)
 
 bool bad(int64_t M, int D, int F, int act, int dtype) {
   return M < 0 || M > (1 << 30) || D < 8 || F < 8 || D % 8 || F % 8 || D > (1 << 20) || F > (1 << 20) || dtype < 0 || dtype > 1 ||
@@ -765,12 +764,12 @@ bool bad(int64_t M, int D, int F, int act, int dtype) {
 }
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
-FfProd prod(const void* P, const void* Q, void* out, int64_t ldp, int64_t ldq, int64_t ldo, int64_t M, int64_t N) {
+FfProd prod(const void* P, const void* Q, void* out, int64_t ldp, int64_t ldq, int64_t M, int64_t N) {
   FfProd r{};
   r.P[0] = r.P[1] = (const char*)P;
   r.Q[0] = r.Q[1] = (const char*)Q;
   r.out = (char*)out;
-  r.ldp = ldp; r.ldq = ldq; r.ldo = ldo; r.M = (int)M; r.N = (int)N;
+  r.ldp = ldp; r.ldq = ldq; r.M = (int)M; r.N = (int)N;
   return r;
 }
 
@@ -779,16 +778,15 @@ void forward(const fluxhip_gated_ff_desc* d, hipStream_t st) {
   const int64_t M = d->M;
   const int D = d->D, F = d->F;
   FfArgs a{};
-  a.pr[0] = prod(d->w_value, d->x, d->hidden, D, d->ldx, F, M, F);
+  a.pr[0] = prod(d->w_value, d->x, d->hidden, D, d->ldx, M, F);
   a.pr[0].P[1] = (const char*)d->w_gate;
   a.nprod = a.nseg = 1; a.K = D; a.act = d->act; a.part = (float*)d->ws;
   a.vout = (char*)d->value; a.gout = (char*)d->gate;
   a.bias[0] = (const char*)d->b_value; a.bias[1] = (const char*)d->b_gate;
-  a.pr[0].ldo = F;
   if (M <= GEMV) launch_gemv<true, H>(a, st);
   else launch<false, false, EPI_UP, H>(a, plan_up(M, D, F), st);
   FfArgs b{};
-  b.pr[0] = prod(d->w_out, d->hidden, d->y, F, F, D, M, D);
+  b.pr[0] = prod(d->w_out, d->hidden, d->y, F, F, M, D);
   b.nprod = b.nseg = 1; b.K = F; b.part = (float*)d->ws; b.bias[0] = (const char*)d->b_out;
   if (M <= GEMV) launch_gemv<false, H>(b, st);
   else launch<false, false, EPI_STORE, H>(b, plan_down(M, D, F), st);
@@ -801,7 +799,7 @@ void backward(const fluxhip_gated_ff_grad_desc* d, hipStream_t st) {
   {
     const Plan p = plan_dh(M, D, F);
     FfArgs a{};
-    a.pr[0] = prod(d->w_out, d->dy, nullptr, F, d->lddy, F, M, F);
+    a.pr[0] = prod(d->w_out, d->dy, nullptr, F, d->lddy, M, F);
     a.nprod = a.nseg = 1; a.K = D; a.act = d->act;
     a.value = (const char*)d->value; a.gate = (const char*)d->gate; a.vout = (char*)d->dvalue; a.gout = (char*)d->dgate;
     a.part = (float*)((char*)d->ws + (d->db_value ? colsum_rows(M, p) * 2 * F * 4 : 0));
@@ -809,7 +807,7 @@ void backward(const fluxhip_gated_ff_grad_desc* d, hipStream_t st) {
     launch<true, false, EPI_DH, H>(a, p, st);
     if (d->db_value) {                                     // dy's columns: few rows are added up by the same launch as they are
       Extra e{d->dy, d->db_out, d->lddy, M, D, 0};
-      if (M > 4 * COLSUM_ROWS) {
+      if (M > 2 * COLSUM_ROWS) {
         float* part = (float*)d->ws + colsum_rows(M, p) * 2 * F;
         hipLaunchKernelGGL((ff_colsum_kernel<H>), dim3((D + 511) / 512, COLSUM_ROWS), dim3(64), 0, st, (const uint16_t*)d->dy, d->lddy, (int)M, D,
                            part);
@@ -820,7 +818,7 @@ void backward(const fluxhip_gated_ff_grad_desc* d, hipStream_t st) {
   }
   if (d->dx) {
     FfArgs a{};
-    a.pr[0] = prod(d->w_value, d->dvalue, d->dx, D, F, D, M, D);
+    a.pr[0] = prod(d->w_value, d->dvalue, d->dx, D, F, M, D);
     a.pr[0].P[1] = (const char*)d->w_gate;
     a.pr[0].Q[1] = (const char*)d->dgate;
     a.nprod = 1; a.nseg = 2; a.K = F; a.part = (float*)d->ws;
@@ -829,10 +827,10 @@ void backward(const fluxhip_gated_ff_grad_desc* d, hipStream_t st) {
   if (d->dw_value || d->dw_out) {                          // all weight gradients in one launch
     FfArgs a{};
     if (d->dw_value) {
-      a.pr[a.nprod++] = prod(d->x, d->dvalue, d->dw_value, d->ldx, F, D, F, D);
-      a.pr[a.nprod++] = prod(d->x, d->dgate, d->dw_gate, d->ldx, F, D, F, D);
+      a.pr[a.nprod++] = prod(d->x, d->dvalue, d->dw_value, d->ldx, F, F, D);
+      a.pr[a.nprod++] = prod(d->x, d->dgate, d->dw_gate, d->ldx, F, F, D);
     }
-    if (d->dw_out) a.pr[a.nprod++] = prod(d->hidden, d->dy, d->dw_out, F, d->lddy, F, D, F);
+    if (d->dw_out) a.pr[a.nprod++] = prod(d->hidden, d->dy, d->dw_out, F, d->lddy, D, F);
     a.nseg = 1; a.K = (int)M; a.part = (float*)d->ws;
     launch<true, true, EPI_STORE, H>(a, a.nprod == 3 ? plan_dw(M, D, F) : a.nprod == 2 ? plan_dw2(M, D, F) : plan_dw1(M, D, F), st);
   }
