@@ -268,6 +268,50 @@ def test_rotary_layouts(dev):
     assert e[0].shape == (B, 0, H, hd) and e[1].shape == (B, 0, K, hd)
 
 
+@pytest.mark.parametrize("M,D,F", [(1, 40, 72), (3, 72, 40), (130, 136, 200), (517, 648, 1288), (1000, 1280, 2568), (2500, 120, 2056)])
+def test_gated_ff_writes_nothing_else(dev, M, D, F):
+    """Every output and the workspace between guard words, which stay; the values are those of the public calls."""
+    from flux_generator_amd import ops
+    from flux_generator_amd._lib import GatedFfDesc, GatedFfGradDesc, load
+    lib = load()
+    t, b = ff_case(M, D, F, BF, True, seed=40)
+    c, cb = {k: v.to(dev) for k, v in t.items()}, [v.to(dev) for v in b]
+    st = torch.cuda.current_stream().cuda_stream
+    ptr = lambda *ts: [q.data_ptr() for q in ts]
+
+    def guarded(*bytes_):
+        offs, n = [], 4096
+        for k in bytes_:
+            offs.append(n)
+            n = -(-(n + k) // 256) * 256 + 4096
+        return torch.full((n,), 0xA5, dtype=torch.uint8, device=dev), offs
+
+    def look(buf, offs, want, ws):
+        keep = torch.ones_like(buf, dtype=torch.bool)
+        for o, w in zip(offs, want):
+            k = w.numel() * 2
+            assert torch.equal(buf[o:o + k].view(BF).view(w.shape), w)
+            keep[o:o + k] = False
+        keep[offs[-1]:offs[-1] + ws] = False
+        assert bool((buf[keep] == 0xA5).all())
+
+    y, sv = ops.gated_ff(c["x"], c["wv"], c["wg"], c["wo"], *cb, act=ops.EPI_SILU, save=True)
+    ws = lib.fluxhip_gated_ff_ws(M, D, F)
+    buf, offs = guarded(*[2 * M * F] * 3, 2 * M * D, ws)
+    at = [buf.data_ptr() + o for o in offs]
+    d = GatedFfDesc(*ptr(c["x"], c["wv"], c["wg"], c["wo"], *cb), *at[:4], M, D, D, F, ops.EPI_SILU, 0, at[4], ws)
+    assert lib.fluxhip_gated_ff(d, st) == 0
+    look(buf, offs, (*sv, y), ws)
+
+    out = ops.gated_ff_backward(c["dy"], c["x"], sv, c["wv"], c["wg"], c["wo"], act=ops.EPI_SILU, bias_grads=True)
+    ws = lib.fluxhip_gated_ff_grad_ws(M, D, F)
+    buf, offs = guarded(*[2 * q.numel() for q in out], *[2 * M * F] * 2, ws)
+    at = [buf.data_ptr() + o for o in offs]
+    d = GatedFfGradDesc(*ptr(c["dy"], c["x"], *sv, c["wv"], c["wg"], c["wo"]), at[7], at[8], *at[:7], M, D, D, D, F, ops.EPI_SILU, 0, at[9], ws)
+    assert lib.fluxhip_gated_ff_grad(d, st) == 0
+    look(buf, offs, (*out, *(buf[o:o + 2 * M * F].view(BF) for o in offs[7:9])), ws)
+
+
 def test_offsets_beyond_32_bits(dev):
     """Tensors of more than 2^32 bytes and 2^31 elements: the last rows are those of a call on them alone."""
     from flux_generator_amd import ops
