@@ -568,7 +568,8 @@ __global__ __launch_bounds__(NF == 4 ? 256 : 512, 2) void ff_gemm_kernel(FfArgs 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no piece outlives the kernel
 }
 
-// adds a split tile's partials in split order and writes it; a block takes one m fragment of each wave's tile
+// adds a split tile's partials in split order and writes it; a block takes one m fragment of each wave's tile.  Few blocks where few
+// rows are: bound by latency, so four splits' loads are in flight (forward of 36 tokens, 1064 -> 240: 16.5 us, with two 21.2)
 template <int NF, int EPI, bool H>
 __global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a) {
   typedef Geo<NF, EPI> G;
@@ -581,7 +582,7 @@ __global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a
   f32x4 acc[NF][1];
   static_for<0, NF>([&](auto i) { acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; });
   const f32x4* p = (const f32x4*)a.part + (((int64_t)tile * a.splits * G::NW + wave) * (NF * MF) + j0) * 64 + lane;
-#pragma unroll 2
+#pragma unroll 4
   for (int z = 0; z < a.splits; ++z) {
     static_for<0, NF>([&](auto i) { acc[i][0] += p[i * MF * 64]; });
     p += (int64_t)G::NW * (NF * MF) * 64;
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a
 // ---- one or two tokens (serving): bound by reading the weights once.  A wave owns one output column - its value and gate row, or
 // its row of the out weight - and reads the rows whole, 1 KiB at a time and eight loads ahead, against the tokens' vectors from
 // L1; products are float32 FMAs.  4096 -> 10240 at one token: 26.8 us for 168 MB (6.3 TB/s), back 15.5 us.  (Three tokens and
-// more: the tiles above with their split along k are faster: 77 us forward at four tokens, 90 this way.)
+// more: the tiles above with their split along k are faster: 56 us forward at four tokens, 90 this way.)
 constexpr int GEMV = 2;
 template <bool DUAL, int MT, bool H>
 __global__ __launch_bounds__(256) void ff_gemv_kernel(FfArgs a) {
