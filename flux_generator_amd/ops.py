@@ -1088,15 +1088,16 @@ def rotary_frequencies(dims, theta: float = 10000.0, scaling: Optional[str] = No
     """(freqs float64 [sum(dims) / 2], scale) for `rotary`: theta^(-2 j / d) over the pairs of every axis width d in `dims` (an int:
     one axis).  For contexts `factor` times the trained length:  "linear" divides every frequency by factor;  "ntk" raises theta to
     theta factor^(d / (d - 2)), which leaves the fastest pair and divides the slowest by factor;  "yarn" divides the pairs that
-    turn fewer than beta_slow times over original_length positions, keeps those above beta_fast, blends linearly (in the pair index)
-    between, and scales by 0.1 ln(factor) + 1."""
+    turn fewer than beta_slow times over original_length positions, keeps those above beta_fast, blends linearly in the pair index
+    between (from the whole index below the first of them, at least 0, to the whole index above the last, at most d - 1 - which
+    lies behind the slowest pair where that turns more than beta_slow times), and scales by 0.1 ln(factor) + 1."""
     dims = [dims] if isinstance(dims, int) else list(dims)
     if not dims or any(d < 2 or d % 2 for d in dims):
         raise FluxHipError("rotary widths must be even and at least 2")
-    if scaling not in (None, "linear", "ntk", "yarn") or factor < 1.0 or theta <= 0.0:
-        raise FluxHipError("scaling must be None, 'linear', 'ntk' or 'yarn', with factor >= 1 and theta > 0")
-    if scaling == "yarn" and (original_length < 1 or not beta_fast > beta_slow > 0):
-        raise FluxHipError("yarn needs original_length >= 1 and beta_fast > beta_slow > 0")
+    if scaling not in (None, "linear", "ntk", "yarn") or not 1.0 <= factor < math.inf or not 0.0 < theta < math.inf:
+        raise FluxHipError("scaling must be None, 'linear', 'ntk' or 'yarn', with finite factor >= 1 and theta > 0")
+    if scaling == "yarn" and not (1 <= original_length < math.inf and math.inf > beta_fast > beta_slow > 0 and theta > 1.0):
+        raise FluxHipError("yarn needs original_length >= 1, beta_fast > beta_slow > 0 and theta > 1")
     parts = []
     for d in dims:
         j = torch.arange(0, d, 2, dtype=torch.float64)
@@ -1108,8 +1109,8 @@ def rotary_frequencies(dims, theta: float = 10000.0, scaling: Optional[str] = No
             f = f / factor
         elif scaling == "yarn":
             pair = lambda turns: d * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
-            lo, hi = max(0, math.floor(pair(beta_fast))), min(d // 2 - 1, math.ceil(pair(beta_slow)))
-            keep = 1 - ((j / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+            lo, hi = max(0, math.floor(pair(beta_fast))), min(d - 1, math.ceil(pair(beta_slow)))
+            keep = 1 - ((j / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1) if pair(beta_slow) >= 0 else torch.zeros_like(j)
             f = f * keep + f / factor * (1 - keep)
         parts.append(f)
     scale = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" and factor > 1.0 else 1.0
