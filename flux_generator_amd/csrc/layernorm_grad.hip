@@ -207,14 +207,16 @@ __global__ __launch_bounds__(64 * WAVES, !PG ? (NCH == 1 ? 6 : 4) : NCH == 1 ? 4
   const float inv = 1.0f / (float)a.D;
   for (; t0 < a.T; t0 += step) {
     const int64_t t = t0 + sub;
-    const float on = t < a.T ? 1.f : 0.f;                 // a repeated row adds nothing to the parameter sums
+    // a repeated row adds nothing to the parameter sums: zeros in its place (its own values times zero would be NaN where the row
+    // holds an infinity)
+    const bool on = !PG || t < a.T;
     typename Elem<T>::raw8 cx[NCH], cd[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      cx[i] = wx[i];
-      cd[i] = wd[i];
+      cx[i] = on ? wx[i] : typename Elem<T>::raw8{};
+      cd[i] = on ? wd[i] : typename Elem<T>::raw8{};
     }
-    const float m = mu, rs = r;
+    const float m = on ? mu : 0.f, rs = on ? r : 0.f;
     if (t0 + step < a.T) fetch(t + step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -227,9 +229,8 @@ __global__ __launch_bounds__(64 * WAVES, !PG ? (NCH == 1 ? 6 : 4) : NCH == 1 ? 4
         s1 += e;
         s2 += e * xh;
         if constexpr (PG) {
-          const float dyo = dy * on;
-          dg[i][j] += dyo * xh;
-          db[i][j] += dyo;
+          dg[i][j] += dy * xh;
+          db[i][j] += dy;
         }
       }
       if constexpr (T < 2) asm volatile("" : "+v"(cx[i]), "+v"(cd[i]));  // unpack again below: half the registers across the reduction

@@ -1,0 +1,59 @@
+"""Adapter-training operators with infinities, NaN and extreme values in their operands, and in place over many rows."""
+import pytest
+import torch
+
+import train_refs as R
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+INF, NAN = float("inf"), float("nan")
+
+
+def rnd(*shape, scale=1.0, mean=0.0, seed=0, dt=BF):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale + mean).to(dt)
+
+
+def D64(t):
+    return t.detach().cpu().double()
+
+
+# ------------------------------------------------------------------------------------------------ LayerNorm
+# (rows, width): one block and several, every number of threads a row, last rounds that leave row groups without a row, and (rows
+# up to 512) sums over the inputs themselves; 9001: rows too wide for registers
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("per", [False, True])
+@pytest.mark.parametrize("T,D", [(5, 64), (1001, 64), (2051, 100), (1003, 771), (517, 1280), (1, 8), (301, 640), (2050, 2560), (1030, 4100), (70, 9001)])
+def test_layernorm_infinities_stay_in_their_row_and_column(dev, T, D, per, dt):
+    from flux_generator_amd import ops
+    B = 2 if per else 1
+    x, dy = rnd(B, T, D, mean=0.5, seed=1, dt=dt).to(dev), rnd(B, T, D, seed=2, dt=dt).to(dev)
+    g = rnd(*((B, D) if per else (D,)), scale=0.2, mean=1.0, seed=3, dt=dt).to(dev)
+    y, mu, r = ops.layernorm(x, g, None)
+    for row in (T - 1, 0, T // 2):
+        c = (7 * row + 3) % D
+        clean = dy.clone()
+        clean[-1, row, c] = 0
+        bad = dy.clone()
+        bad[-1, row, c] = INF
+        cx, cg, cb = ops.layernorm_backward(clean, x, mu, r, g)
+        bx, bg, bb = ops.layernorm_backward(bad, x, mu, r, g)
+        other = torch.ones(B, T, dtype=torch.bool, device=dev)
+        other[-1, row] = False
+        assert torch.equal(bx[other], cx[other]) and not bool(bx[-1, row].isfinite().any())
+        col = torch.ones_like(g, dtype=torch.bool)
+        col.view(-1, D)[-1, c] = False
+        assert torch.equal(bg[col], cg[col]) and torch.equal(bb[col], cb[col])
+        xh = (x[-1, row, c].double() - mu[-1, row]) * r[-1, row]
+        assert float(bb.view(-1, D)[-1, c]) == INF, (row, bb.view(-1, D)[-1, c])
+        assert float(bg.view(-1, D)[-1, c]) == (INF if float(xh) > 0 else -INF), (row, float(xh))
+        # an activation that overflowed: its row's outputs and the weight's gradient are lost, everything else stands
+        hot = x.clone()
+        hot[-1, row, c] = NAN
+        hy, hm, hr = ops.layernorm(hot, g, None)
+        assert torch.equal(hy[other], y[other]) and bool(hy[-1, row].isnan().all()) and torch.equal(hm[other], mu[other])
+        hx, hg, hb = ops.layernorm_backward(dy, hot, hm, hr, g)
+        gx, gg, gb = ops.layernorm_backward(dy, x, mu, r, g)
+        assert torch.equal(hx[other], gx[other]) and torch.equal(hb, gb)
+        assert bool(hg.view(-1, D)[-1].isnan().all()) and torch.equal(hg.view(-1, D)[:-1], gg.view(-1, D)[:-1])
