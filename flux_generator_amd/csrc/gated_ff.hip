@@ -155,7 +155,7 @@ DEVINL void act_grad(float x, float& f, float& df) {
     df = p * (1.0f + x * (1.0f - p));
   } else if constexpr (ACT == FLUXHIP_EPI_GELU_TANH) {
     constexpr float c0 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, c1 = c0 * 0.044715f;
-    const float x2 = x * x;
+    const float x2 = fminf(x * x, 1e30f);                  // (an infinite square would meet 1 - p = 0 below)
     const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * __builtin_fmaf(x2, c1, c0)));
     f = x * p;
     df = p + f * (1.0f - p) * (1.5957691216057308f * __builtin_fmaf(x2, 0.134145f, 1.0f));

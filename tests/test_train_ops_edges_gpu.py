@@ -57,3 +57,23 @@ def test_layernorm_infinities_stay_in_their_row_and_column(dev, T, D, per, dt):
         gx, gg, gb = ops.layernorm_backward(dy, x, mu, r, g)
         assert torch.equal(hx[other], gx[other]) and torch.equal(hb, gb)
         assert bool(hg.view(-1, D)[-1].isnan().all()) and torch.equal(hg.view(-1, D)[:-1], gg.view(-1, D)[:-1])
+
+
+# ------------------------------------------------------------------------------------------------ gated feed-forward
+@pytest.mark.parametrize("kind,name", [("erf", "EPI_GELU_ERF"), ("tanh", "EPI_GELU_TANH"), ("silu", "EPI_SILU")])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_gated_ff_gradient_over_the_whole_range_of_gates(dev, kind, name, dt):
+    """One token whose gates run over everything finite: the derivative is 0 or 1 far out, never NaN."""
+    from flux_generator_amd import ops
+    big = [1e-30, 1e-6, 0.3, 2.0, 5.5, 12.0, 40.0, 90.0, 1e3, 6e4] + ([1e9, 1e12, 1e18, 1.8e19, 1.9e19, 1e20, 1e30, 3.3e38] if dt == BF else [])
+    gate = torch.tensor([s * b for b in big for s in (1, -1)] + [0.0] * (40 - 2 * len(big)), dtype=dt)[None]
+    F, D = gate.shape[1], 64
+    x, dy, value = rnd(1, D, seed=1, dt=dt), rnd(1, D, seed=2, dt=dt), rnd(1, F, seed=3, dt=dt)
+    wv, wg, wo = rnd(F, D, scale=1e-3, seed=4, dt=dt), rnd(F, D, scale=D ** -0.5, seed=5, dt=dt), rnd(D, F, scale=1e-3, seed=6, dt=dt)
+    hidden = torch.zeros(1, F, dtype=dt)
+    c = lambda t: t.to(dev)
+    out = ops.gated_ff_backward(c(dy), c(x), (c(value), c(gate), c(hidden)), c(wv), c(wg), c(wo), act=getattr(ops, name), bias_grads=True)
+    pairs = R.ff_backward_bound(D64(dy), D64(x), D64(value), D64(gate), D64(hidden), D64(wv), D64(wg), D64(wo), kind, dt)
+    for what, got, pair in zip(("dx", "dw_value", "dw_gate", "dw_out", "db_value", "db_gate", "db_out"), out, pairs):
+        assert bool(got.isfinite().all()), (what, gate[0, got.isfinite().logical_not().nonzero()[0, 0]])
+        R.check(got, pair, what)
