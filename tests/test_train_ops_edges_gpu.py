@@ -77,3 +77,62 @@ def test_gated_ff_gradient_over_the_whole_range_of_gates(dev, kind, name, dt):
     for what, got, pair in zip(("dx", "dw_value", "dw_gate", "dw_out", "db_value", "db_gate", "db_out"), out, pairs):
         assert bool(got.isfinite().all()), (what, gate[0, got.isfinite().logical_not().nonzero()[0, 0]])
         R.check(got, pair, what)
+
+
+@pytest.mark.parametrize("M,D,F", [(2, 64, 136), (5, 72, 40), (130, 128, 384), (1000, 1280, 2568), (2947, 952, 2728)])
+def test_gated_ff_keeps_rows_apart(dev, M, D, F):
+    """A token that is NaN, and one whose gradient is infinite, leave every other token's results as they are."""
+    from flux_generator_amd import ops
+    x, dy = rnd(M, D, seed=1).to(dev), rnd(M, D, seed=2).to(dev)
+    W = [t.to(dev) for t in (rnd(F, D, scale=D ** -0.5, seed=3), rnd(F, D, scale=D ** -0.5, seed=4), rnd(D, F, scale=F ** -0.5, seed=5))]
+    y, s = ops.gated_ff(x, *W, save=True)
+    dx = ops.gated_ff_backward(dy, x, s, *W)[0]
+    for row in {0, M // 2, M - 1}:
+        other = torch.arange(M, device=dev) != row
+        hot = x.clone()
+        hot[row, D // 2] = NAN
+        hy, hs = ops.gated_ff(hot, *W, save=True)
+        assert bool(hy[row].isnan().all()) and torch.equal(hy[other], y[other])
+        assert all(torch.equal(p[other], q[other]) and bool(p[row].isnan().all()) for p, q in zip(hs, s))
+        bad = dy.clone()
+        bad[row, D // 2] = INF
+        bx = ops.gated_ff_backward(bad, x, s, *W)[0]
+        assert torch.equal(bx[other], dx[other]) and not bool(bx[row].isfinite().any())
+
+
+# ------------------------------------------------------------------------------------------------ rotary
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("inter", [True, False])
+def test_rotary_keeps_pairs_apart(dev, inter, dt):
+    from flux_generator_amd import ops
+    B, T, H, K, hd, rot = 2, 37, 5, 2, 84, 44
+    q, k = rnd(B, T, H, hd, seed=1, dt=dt).to(dev), rnd(B, T, K, hd, seed=2, dt=dt).to(dev)
+    freqs, _ = ops.rotary_frequencies(rot, device=dev)
+    pos = torch.arange(T, device=dev)
+    want = ops.rotary(q, k, pos, freqs, interleaved=inter)
+    for col in (0, 1, 9, 21, 22, 43, 44, 83):
+        mate = col if col >= rot else col ^ 1 if inter else (col + rot // 2) % rot
+        bad = q.clone()
+        bad[1, 5, 3, col] = NAN
+        got = ops.rotary(bad, k, pos, freqs, interleaved=inter)
+        assert torch.equal(got[1], want[1]) and bool(got[0][1, 5, 3, [col, mate]].isnan().all())
+        keep = torch.ones_like(q, dtype=torch.bool)
+        keep[1, 5, 3, [col, mate]] = False
+        assert torch.equal(got[0][keep], want[0][keep]), col
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("inter", [True, False])
+@pytest.mark.parametrize("rot,hd", [(30, 48), (44, 48), (26, 84), (1030, 1031), (2054, 2060)])
+def test_rotary_in_place_over_many_tokens(dev, rot, hd, inter, dt):
+    """Widths whose last vector is moved back, with more (token, head) items than a block takes at once."""
+    from flux_generator_amd import ops
+    B, T, H, K = (2, 5000, 24, 8) if hd < 100 else (2, 60, 24, 8)
+    qkv = rnd(B, T, (H + 2 * K) * hd, seed=1, dt=dt).to(dev)
+    q, k = qkv[..., : H * hd].unflatten(-1, (H, hd)), qkv[..., H * hd: (H + K) * hd].unflatten(-1, (K, hd))
+    values = qkv[..., (H + K) * hd:].clone()
+    freqs, _ = ops.rotary_frequencies(rot, device=dev)
+    pos = torch.arange(T, device=dev) + 5
+    want = ops.rotary(q, k, pos, freqs, interleaved=inter)
+    a, b = ops.rotary(q, k, pos, freqs, interleaved=inter, out=(q, k))
+    assert a is q and torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(qkv[..., (H + K) * hd:], values)
