@@ -861,7 +861,8 @@ extern "C" int fluxhip_gated_ff(const fluxhip_gated_ff_desc* d, void* stream) {
   if (!d->x || !d->w_value || !d->w_gate || !d->w_out || !d->hidden || !d->y || !d->value != !d->gate || !d->b_value != !d->b_gate ||
       d->ldx < d->D || d->ldx % 8 || d->ldx > (1 << 21) || (need && (!d->ws || d->ws_bytes < need)))
     return FLUXHIP_EINVAL;
-  for (const void* p : {d->x, d->w_value, d->w_gate, d->w_out, (const void*)d->hidden, (const void*)d->y, (const void*)d->ws})
+  for (const void* p : {d->x, d->w_value, d->w_gate, d->w_out, (const void*)d->value, (const void*)d->gate, (const void*)d->hidden,
+                        (const void*)d->y, (const void*)d->ws})
     if (misaligned(p)) return FLUXHIP_EINVAL;
   if (d->dtype == 1) forward<true>(d, (hipStream_t)stream);
   else forward<false>(d, (hipStream_t)stream);
@@ -878,7 +879,7 @@ extern "C" int fluxhip_gated_ff_grad(const fluxhip_gated_ff_grad_desc* d, void* 
       !d->ws || d->ws_bytes < need)
     return FLUXHIP_EINVAL;
   for (const void* p : {d->dy, d->x, d->value, d->gate, d->hidden, d->w_value, d->w_gate, d->w_out, (const void*)d->dvalue, (const void*)d->dgate,
-                        (const void*)d->ws})
+                        (const void*)d->dx, (const void*)d->dw_value, (const void*)d->dw_gate, (const void*)d->dw_out, (const void*)d->ws})
     if (misaligned(p)) return FLUXHIP_EINVAL;
   if (d->dtype == 1) backward<true>(d, (hipStream_t)stream);
   else backward<false>(d, (hipStream_t)stream);

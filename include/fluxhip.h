@@ -569,7 +569,7 @@ int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream);
 
 /* Gated feed-forward block: value = x Wv^T + bv, gate = x Wg^T + bg, hidden = value act(gate), y = hidden Wo^T + bo
  * (stable_diffusion/.../unet.py:74-78 and its linear3; flux/t5.py:163-177).  Weights [F][D], [F][D], [D][F] row-major, D % 8 == 0,
- * F % 8 == 0, every pointer 16-byte aligned, ldx % 8 == 0.  act: FLUXHIP_EPI_GELU_TANH, FLUXHIP_EPI_GELU_ERF or
+ * F % 8 == 0, every matrix and ws 16-byte aligned (biases: element alignment), ldx % 8 == 0.  act: FLUXHIP_EPI_GELU_TANH, FLUXHIP_EPI_GELU_ERF or
  * FLUXHIP_EPI_SILU.  dtype: bf16 or f16; products accumulate in float32; value, gate and hidden are rounded to dtype (hidden is
  * formed from the unrounded two).  value / gate may be NULL (both); hidden [M][F] is always written. */
 typedef struct fluxhip_gated_ff_desc {
@@ -587,7 +587,8 @@ int fluxhip_gated_ff(const fluxhip_gated_ff_desc* d, void* stream);
 /* Its gradient from dy and the saved value, gate (and hidden, for dw_out):
  *   dh = dy Wo, dvalue = dh act(gate), dgate = dh value act'(gate)   (rounded to dtype, [M][F] each, written for the products below)
  *   dx = dvalue Wv + dgate Wg, dWv = dvalue^T x, dWg = dgate^T x, dWo = dy^T hidden, db = column sums (db_value, db_gate of the unrounded values).
- * Outputs that are NULL are not computed (dw_value and dw_gate together, the three db together).  ldx, lddy % 8 == 0. */
+ * Outputs that are NULL are not computed (dw_value and dw_gate together, the three db together).  ldx, lddy % 8 == 0, every matrix -
+ * dx and the dw too - and ws 16-byte aligned. */
 typedef struct fluxhip_gated_ff_grad_desc {
   const void *dy, *x, *value, *gate, *hidden, *w_value, *w_gate, *w_out;
   void *dvalue, *dgate;

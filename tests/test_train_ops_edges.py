@@ -59,3 +59,26 @@ def test_frequency_refusals(bad):
     from flux_generator_amd import ops
     with pytest.raises(ops.FluxHipError):
         ops.rotary_frequencies(16, device="cpu", **bad)
+
+
+def test_gated_ff_entry_points_refuse_misaligned_outputs():
+    """Every tensor that the kernels move in 16-byte pieces must lie at 16 bytes: the outputs as well (host code only)."""
+    import ctypes
+    from flux_generator_amd import _lib, ops
+    lib = _lib.load()
+    M, D, F = 5, 16, 24
+    n = lib.fluxhip_gated_ff_ws(M, D, F)
+    for name in ("x", "w_value", "w_gate", "w_out", "value", "gate", "hidden", "y", "ws"):
+        d = _lib.GatedFfDesc()
+        for k in ("x", "w_value", "w_gate", "w_out", "value", "gate", "hidden", "y", "ws"):
+            setattr(d, k, 4096 + (8 if k == name else 0))
+        d.M, d.ldx, d.D, d.F, d.act, d.ws_bytes = M, D, D, F, ops.EPI_SILU, n
+        assert lib.fluxhip_gated_ff(ctypes.byref(d), None) == -1, name
+    n = lib.fluxhip_gated_ff_grad_ws(M, D, F)
+    names = ("dy", "x", "value", "gate", "hidden", "w_value", "w_gate", "w_out", "dvalue", "dgate", "dx", "dw_value", "dw_gate", "dw_out", "ws")
+    for name in names:
+        d = _lib.GatedFfGradDesc()
+        for k in names:
+            setattr(d, k, 4096 + (8 if k == name else 0))
+        d.M, d.ldx, d.lddy, d.D, d.F, d.act, d.ws_bytes = M, D, D, D, F, ops.EPI_SILU, n
+        assert lib.fluxhip_gated_ff_grad(ctypes.byref(d), None) == -1, name
