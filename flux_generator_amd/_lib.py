@@ -179,6 +179,7 @@ SIGNATURES = {
     "fluxhip_layernorm_grad": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
                                        c_int, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p,
                                        c_int64, c_void_p]),
+    "fluxhip_rotary_overlap": (c_int, [C.POINTER(RotaryDesc)]),
     "fluxhip_rotary": (c_int, [C.POINTER(RotaryDesc), c_void_p]),
     "fluxhip_gated_ff_ws": (c_int64, [c_int64, c_int, c_int]),
     "fluxhip_gated_ff": (c_int, [C.POINTER(GatedFfDesc), c_void_p]),

@@ -185,7 +185,77 @@ void launch(const RopeArgs& a, int interleaved, int inverse, dim3 grid, size_t l
   }
 }
 
+// ---- what an output may share with the inputs (host)
+struct View {                          // a tensor's bytes: first address, and the dimensions that move, the widest stride first
+  int64_t at = 0, stride[4], n[4];
+  int dims = 0, e = 0;
+  bool repeats = false;                // several elements at one address
+  View(const void* p, const int64_t* strides, int64_t B, int64_t T, int64_t H, int64_t hd, int size) : at((int64_t)p), e(size) {
+    const int64_t s[4] = {strides[0] * size, strides[1] * size, strides[2] * size, size}, c[4] = {B, T, H, hd};
+    for (int i = 0; i < 4; ++i) {
+      if (c[i] <= 1) continue;
+      if (s[i] == 0) { repeats = true; continue; }
+      if (s[i] < 0) at += s[i] * (c[i] - 1);
+      int j = dims++;
+      for (; j > 0 && stride[j - 1] < llabs(s[i]); --j) stride[j] = stride[j - 1], n[j] = n[j - 1];
+      stride[j] = llabs(s[i]);
+      n[j] = c[i];
+    }
+    __int128 inside = e;
+    for (int i = dims; i-- > 0;) {     // each stride has to pass over all that lies inside it
+      repeats |= stride[i] < inside;
+      inside += (__int128)stride[i] * (n[i] - 1);
+    }
+  }
+  bool operator==(const View& o) const {
+    bool same = at == o.at && dims == o.dims;
+    for (int i = 0; same && i < dims; ++i) same = stride[i] == o.stride[i] && n[i] == o.n[i];
+    return same;
+  }
+  // bytes from the first to behind the last, of the dimensions from the d-th with strides below `below`
+  __int128 length(int d, __int128 below) const {
+    __int128 l = e;
+    for (int i = d; i < dims; ++i) l += stride[i] < below ? (__int128)stride[i] * (n[i] - 1) : 0;
+    return l;
+  }
+  bool multiple(int d, int64_t period) const {
+    bool ok = true;
+    for (int i = d; i < dims; ++i) ok &= stride[i] < period || stride[i] % period == 0;
+    return ok;
+  }
+};
+// Whether two views provably share no byte: one ends in front of the other, or they lie in different columns of a common period (the
+// heads of a fused projection), sample by sample where their widest strides agree and no sample reaches into the next.
+bool apart(const View& a, const View& b) {
+  const __int128 all = (__int128)1 << 100;
+  const int64_t gap = b.at - a.at;
+  for (int d = 0;; ++d) {
+    const __int128 la = a.length(d, all), lb = b.length(d, all);
+    if (gap >= la || -gap >= lb) return true;
+    for (const View* v : {&a, &b})
+      for (int i = d; i < v->dims; ++i) {
+        const int64_t period = v->stride[i], m = (gap % period + period) % period;
+        if (a.multiple(d, period) && b.multiple(d, period) && m >= a.length(d, period) && m + b.length(d, period) <= period) return true;
+      }
+    if (d >= a.dims || d >= b.dims || a.stride[d] != b.stride[d]) return false;
+    const __int128 ia = a.length(d + 1, all), ib = gap + b.length(d + 1, all);
+    if ((ia > ib ? ia : ib) - (gap < 0 ? gap : 0) > a.stride[d]) return false;
+  }
+}
+
 }  // namespace
+
+extern "C" int fluxhip_rotary_overlap(const fluxhip_rotary_desc* d) {
+  if (!d) return FLUXHIP_EINVAL;
+  const int e = d->dtype == 2 ? 4 : 2;
+  const View q(d->q, d->q_strides, d->B, d->T, d->H, d->hd, e), qo(d->q_out, d->qo_strides, d->B, d->T, d->H, d->hd, e);
+  const View k(d->k, d->k_strides, d->B, d->T, d->K, d->hd, e), ko(d->k_out, d->ko_strides, d->B, d->T, d->K, d->hd, e);
+  if (d->B * d->T == 0) return 0;
+  if ((d->H && qo.repeats) || (d->K && ko.repeats)) return 3;
+  if (d->H && !(qo == q) && !apart(qo, q)) return 1;
+  if (d->K && !(ko == k) && !apart(ko, k)) return 2;
+  return d->H && d->K && !(apart(qo, ko) && apart(qo, k) && apart(q, ko)) ? 4 : 0;
+}
 
 extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   if (!d || d->B < 0 || d->B > (1ll << 32) || d->T < 0 || d->T > (1 << 30) || d->H < 0 || d->K < 0 || d->hd < 1 || d->hd > 4096 ||
@@ -202,7 +272,7 @@ extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   const int64_t ntok = d->B * d->T;
   if (ntok == 0 || d->H + d->K == 0) return FLUXHIP_OK;
   if (d->H > 4096 || d->K > 4096 || !d->positions || !d->freqs ||
-      (d->H && (!d->q || !d->q_out)) || (d->K && (!d->k || !d->k_out))) return FLUXHIP_EINVAL;
+      (d->H && (!d->q || !d->q_out)) || (d->K && (!d->k || !d->k_out)) || fluxhip_rotary_overlap(d)) return FLUXHIP_EINVAL;
   RopeArgs a{};
   a.q = {d->q, d->q_out, d->q_strides[0], d->q_strides[1], d->q_strides[2], d->qo_strides[0], d->qo_strides[1], d->qo_strides[2]};
   a.k = {d->k, d->k_out, d->k_strides[0], d->k_strides[1], d->k_strides[2], d->ko_strides[0], d->ko_strides[1], d->ko_strides[2]};

@@ -1160,13 +1160,15 @@ def _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, inverse, out):
     if k is not None:
         ko, ks, kos = place(k, outs[1], "k")
         K, kp, kop = k.shape[2], k.data_ptr(), ko.data_ptr()
-    if out is not None and k is not None and q.numel() and k.numel() and \
-            (kop == qo.data_ptr() or kop == q.data_ptr() or kp == qo.data_ptr()):
-        raise FluxHipError("out must give q and k memory of their own")
-    st = _launch_stream((q, "q"), (k, "k"), (positions, "positions"), (freqs, "freqs"), (qo, "out"), (ko, "out"))
     d = RotaryDesc(q.data_ptr(), kp, qo.data_ptr(), kop, qs, ks, qos, kos, positions.data_ptr(), freqs.data_ptr(), (pb, pt), B, T, H, K, hd, rot,
                    interleaved, inverse, positions.dtype == torch.int64, na, tuple([w // 2 for w in dims]), _DT[q.dtype], scale)
-    _check(_lib.load().fluxhip_rotary(d, st), "fluxhip_rotary")
+    lib = _lib.load()
+    met = lib.fluxhip_rotary_overlap(d) if out is not None else 0
+    if met:
+        raise FluxHipError(("out must be q itself or not overlap it", "out must be k itself or not overlap it", "out must not overlap itself",
+                            "out must give q and k memory of their own")[met - 1])
+    st = _launch_stream((q, "q"), (k, "k"), (positions, "positions"), (freqs, "freqs"), (qo, "out"), (ko, "out"))
+    _check(lib.fluxhip_rotary(d, st), "fluxhip_rotary")
     return qo if k is None else (qo, ko)
 
 
@@ -1174,7 +1176,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
            interleaved: bool = True, scale: float = 1.0, out=None):
     """Rotary positions on q [B, T, H, head_dim] and k [B, T, K, head_dim] (or None) in one launch -> (q', k') (or q').  Any strides
     with a contiguous last dimension (transposed heads, slices of a fused projection); out: tensors to write, which may be q and k
-    themselves but not overlap them otherwise.  positions [T] or [B, T] integers, with axes_dim of several axes [T, axes] or [B, T, axes]; freqs, scale:
+    themselves but are refused unless they provably lie apart from them otherwise.  positions [T] or [B, T] integers, with axes_dim of several axes [T, axes] or [B, T, axes]; freqs, scale:
     rotary_frequencies.  The first 2 len(freqs) columns turn - pairs (2j, 2j + 1) when interleaved, else (j, j + half) -, the rest is
     copied.  Angles are formed in 64 bits."""
     return _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, False, out)

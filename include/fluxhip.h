@@ -565,6 +565,10 @@ typedef struct fluxhip_rotary_desc {
   int32_t dtype;           /* FLUXHIP_DT_*                                                                     */
   float scale;
 } fluxhip_rotary_desc;
+/* Host only: whether the outputs may be written as `d` says.  0: each is its input or provably lies apart from it, has one element
+ * an address, and q and k have memory of their own; 1 / 2: q_out / k_out overlaps its input; 3: an output overlaps itself;
+ * 4: q and k meet.  fluxhip_rotary refuses whatever is not 0. */
+int fluxhip_rotary_overlap(const fluxhip_rotary_desc* d);
 int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream);
 
 /* Gated feed-forward block: value = x Wv^T + bv, gate = x Wg^T + bg, hidden = value act(gate), y = hidden Wo^T + bo

@@ -82,3 +82,117 @@ def test_gated_ff_entry_points_refuse_misaligned_outputs():
             setattr(d, k, 4096 + (8 if k == name else 0))
         d.M, d.ldx, d.lddy, d.D, d.F, d.act, d.ws_bytes = M, D, D, D, F, ops.EPI_SILU, n
         assert lib.fluxhip_gated_ff_grad(ctypes.byref(d), None) == -1, name
+
+
+def _rotary_args(T=6, rot=8):
+    return torch.arange(T), torch.ones(rot // 2, dtype=F64)
+
+
+def _accepted(q, k, out, T=6):
+    """Every check of the arguments passes: what stops the call is that these are host tensors."""
+    from flux_generator_amd import ops
+    p, f = _rotary_args(T)
+    for fn in (ops.rotary, ops.rotary_backward):
+        with pytest.raises(ops.FluxHipError, match="device tensors"):
+            fn(q, k, p, f, out=out)
+
+
+def _refused(q, k, out, match, T=6):
+    from flux_generator_amd import ops
+    p, f = _rotary_args(T)
+    for fn in (ops.rotary, ops.rotary_backward):
+        with pytest.raises(ops.FluxHipError, match=match):
+            fn(q, k, p, f, out=out)
+
+
+def test_rotary_outputs_that_overlap_are_refused():
+    B, T, H, hd = 2, 6, 4, 8
+    n = B * T * H * hd
+    for step in (1, hd, H * hd):                        # an output shifted against its input
+        buf = torch.zeros(n + step)
+        q, o = buf[:n].view(B, T, H, hd), buf[step:].view(B, T, H, hd)
+        _refused(q, None, o, "q itself")
+        _refused(o, None, q, "q itself")
+        _refused(torch.zeros(B, T, H, hd), q, (torch.zeros(B, T, H, hd), o), "k itself")
+        _refused(q, torch.zeros(B, T, H, hd), (torch.zeros(B, T, H, hd), o), "memory of their own")
+        _refused(torch.zeros(B, T, H, hd), torch.zeros(B, T, H, hd), (q, o), "memory of their own")
+    buf = torch.zeros(n)                                # the input's memory with other strides
+    _refused(buf.view(B, T, H, hd), None, buf.view(B, H, T, hd).transpose(1, 2), "q itself")
+    _refused(buf.view(B, T, H, hd), None, buf.view(T, B, H, hd).transpose(0, 1), "q itself")
+    _refused(torch.zeros(B, T, H, hd), buf.view(B, T, H, hd), (buf.view(B, H, T, hd).transpose(1, 2), torch.zeros(B, T, H, hd)), "memory of their own")
+    _refused(buf.view(B, T, H, hd), buf.view(B, T, H, hd)[:, :, 1:3], (buf.view(B, T, H, hd), buf.view(B, T, H, hd)[:, :, 1:3]), "memory of their own")
+    qkv = torch.zeros(B, T, 3 * H, hd)                  # heads of a fused projection, one too many
+    _refused(qkv[:, :, :H + 1], qkv[:, :, H:2 * H], (qkv[:, :, :H + 1], qkv[:, :, H:2 * H]), "memory of their own")
+    wide = torch.zeros(4 * n)                           # an output that meets itself
+    _refused(torch.zeros(B, T, H, hd), None, wide.as_strided((B, T, H, hd), (T * H * hd, hd, hd, 1)), "overlap itself")
+    _refused(torch.zeros(B, T, H, hd), None, wide.as_strided((B, T, H, hd), (hd, H * hd, hd, 1)), "overlap itself")
+
+
+def test_rotary_outputs_that_do_not_overlap_are_accepted():
+    B, T, H, K, hd = 2, 6, 4, 2, 8
+    z = lambda *s: torch.zeros(*s)
+    q, k = z(B, T, H, hd), z(B, T, K, hd)
+    _accepted(q, k, (q, k))
+    _accepted(q, k, (z(B, T, H, hd), k))
+    _accepted(q, k, (q, z(B, K, T, hd).transpose(1, 2)))
+    _accepted(q, None, q)
+    _accepted(q, None, (q, None))
+    _accepted(z(1, T, 1, hd).expand(B, T, H, hd), None, q)
+    for qkv in (z(B, T, H + 2 * K, hd), z(B, T + 5, H + 2 * K, hd)[:, 5:], z(T, B, H + 2 * K, hd).transpose(0, 1), z(B, T, H + 2 * K, hd + 3)[..., 3:]):
+        a, b, v = qkv[:, :, :H], qkv[:, :, H:H + K], qkv[:, :, H + K:]
+        _accepted(a, b, (a, b))                         # q and k inside one projection
+        _accepted(a, b, (a, v))                         # .. k written over the values
+        _accepted(q, b, (a, v))
+    for five, d in ((z(B, T, 3, H, hd), 2), (z(B, T, H, 3, hd), 3), (z(B, 3, H, T, hd).permute(0, 3, 2, 1, 4), 3), (z(3, B, T, H, hd).movedim(0, 2), 2)):
+        a, b = five.select(d, 0), five.select(d, 1)
+        assert a.shape == (B, T, H, hd)
+        _accepted(a, b, (a, b))
+        _accepted(a, None, b)
+    flat = z(B * (T * H * hd + 5) + T * K * hd + 5)     # samples apart by what is no multiple of a row
+    a = flat.as_strided((B, T, H, hd), (T * H * hd + 5, H * hd, hd, 1))
+    _accepted(a, None, a)
+    packed = z(B * (T * (H + K) * hd + 5))
+    a = packed.as_strided((B, T, H, hd), (T * (H + K) * hd + 5, (H + K) * hd, hd, 1))
+    b = packed.as_strided((B, T, K, hd), (T * (H + K) * hd + 5, (H + K) * hd, hd, 1), H * hd)
+    _accepted(a, b, (a, b))
+    cols = z(B, T, H, 2 * hd)                           # halves of wider heads
+    _accepted(cols[..., :hd], cols[..., hd:], (cols[..., :hd], cols[..., hd:]))
+    _accepted(z(B, 0, H, hd), z(B, 0, K, hd), (z(B, 0, H, hd), z(B, 0, K, hd)), T=0)
+    _accepted(q[:, :, :0], k, (q[:, :, :0], k))
+
+
+def test_rotary_overlap_is_judged_as_by_the_addresses():
+    """Random pairs of views of one small buffer: an output that is let through shares no element with its input but as that input
+    itself, and holds each of its elements once; most of those that lie apart are let through."""
+    import ctypes
+    import random
+    from flux_generator_amd import _lib
+    lib, rng = _lib.load(), random.Random(0)
+    index = torch.arange(8192)
+    count = dict(met=0, apart=0, proved=0, same=0, inside=0)
+    for _ in range(20000):
+        def strides():
+            return [rng.choice((0, 1, 2, 3, 4, 5, 8, 12, 16, 32, 48, 96, 100)) for _ in range(3)]
+        shape, sa, sb = [rng.randint(1, 4) for _ in range(4)], strides(), strides()
+        at, bt = rng.randint(0, 60), rng.randint(0, 60)
+        if rng.random() < 0.6:
+            sb = sa
+        if rng.random() < 0.05:
+            sb, bt = sa, at
+        ia, ib = (index.as_strided(shape, s + [1], o).reshape(-1).tolist() for s, o in ((sa, at), (sb, bt)))
+        d = _lib.RotaryDesc()
+        d.B, d.T, d.H, d.hd = shape
+        d.dtype = rng.choice((0, 2))
+        e = 4 if d.dtype == 2 else 2
+        d.q, d.q_out, d.q_strides, d.qo_strides = (1 << 20) + e * at, (1 << 20) + e * bt, tuple(sa), tuple(sb)
+        said, once, met = lib.fluxhip_rotary_overlap(ctypes.byref(d)), len(set(ib)) == len(ib), bool(set(ia) & set(ib))
+        if said == 0:
+            assert once and (not met or ia == ib), (shape, sa, at, sb, bt)
+        if once and ia == ib and said != 3:
+            assert said == 0
+        count["inside"] += not once
+        count["same"] += ia == ib
+        count["met"] += once and met and ia != ib
+        count["apart"] += once and not met
+        count["proved"] += once and not met and said == 0
+    assert all(n > 200 for n in count.values()) and count["proved"] > 0.5 * count["apart"], count
