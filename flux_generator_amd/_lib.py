@@ -223,14 +223,16 @@ def load() -> C.CDLL:
     # FLUXHIP_LIB_AB=1 (tools/lib_ab.py: timing an OLDER build of the library against the current one through the current
     # Python host code) tolerates symbols that build does not have yet and its ABI version; never set it for product runs
     ab = bool(os.environ.get("FLUXHIP_LIB_AB")) and "FLUXHIP_LIB" in os.environ
-    for name, (res, args) in SIGNATURES.items():
-        if ab and not hasattr(lib, name):
-            continue
-        fn = getattr(lib, name)  # AttributeError if the symbol is not exported
-        fn.restype = res
-        fn.argtypes = args
     if lib.fluxhip_abi_version() != 9 and not ab:
         raise RuntimeError("libfluxhip ABI version mismatch")
+    missing = [name for name in SIGNATURES if not hasattr(lib, name)]
+    if missing and not ab:
+        raise RuntimeError(f"{LIB_PATH} lacks {', '.join(missing)}: it was built from older sources, build it again")
+    for name, (res, args) in SIGNATURES.items():
+        if name not in missing:
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
     if lib.fluxhip_arch() != b"gfx950":
         raise RuntimeError("libfluxhip was not built for gfx950")
     _lib = lib

@@ -196,3 +196,22 @@ def test_rotary_overlap_is_judged_as_by_the_addresses():
         count["apart"] += once and not met
         count["proved"] += once and not met and said == 0
     assert all(n > 200 for n in count.values()) and count["proved"] > 0.5 * count["apart"], count
+
+
+@pytest.mark.parametrize("version,match", [(9, "lacks fluxhip_.*build"), (8, "ABI version mismatch")])
+def test_a_library_of_older_sources_is_named_as_such(tmp_path, monkeypatch, version, match):
+    """A build from before a symbol came in (same ABI number), and one of another ABI number: each says so."""
+    import shutil
+    import subprocess
+    from flux_generator_amd import _lib
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if not cc:
+        pytest.skip("no C compiler")
+    (tmp_path / "old.c").write_text(f'int fluxhip_abi_version(void) {{ return {version}; }}\nconst char* fluxhip_arch(void) {{ return "gfx950"; }}\n')
+    subprocess.run([cc, "-shared", "-fPIC", "-o", str(tmp_path / "old.so"), str(tmp_path / "old.c")], check=True)
+    monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "old.so")
+    monkeypatch.setattr(_lib, "_lib", None)
+    monkeypatch.delenv("FLUXHIP_LIB_AB", raising=False)
+    with pytest.raises(RuntimeError, match=match):
+        _lib.load()
+    assert _lib._lib is None
