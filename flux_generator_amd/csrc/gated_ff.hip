@@ -22,7 +22,6 @@ namespace {
 constexpr int BK = 64;
 constexpr uint32_t OOB = 0xFFFFFFF0u;                      // a buffer offset that fails every range check: the load writes zeros
 typedef __attribute__((ext_vector_type(4))) short s16x4;
-typedef __attribute__((address_space(3))) char lds_char;
 
 enum { EPI_STORE = 0, EPI_UP = 1, EPI_DH = 2 };
 

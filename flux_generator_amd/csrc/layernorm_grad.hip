@@ -402,16 +402,19 @@ int64_t partials(int64_t B, int64_t T, int D, Shape s) {
   return n > (groups + 3) / 4 ? (groups + 3) / 4 : n;
 }
 
-#define LN_DISPATCH(KERNEL, ...)                                              \
+// MANY: two or three chunks a lane are built where pick takes them - 16-bit types, whole chunks, no parameter gradient
+#define LN_DISPATCH(KERNEL, MANY, ...)                                        \
   if (s.nt == 16) KERNEL(16, 1, __VA_ARGS__);                                 \
   else if (s.nt == 64 && s.nch == 1) KERNEL(64, 1, __VA_ARGS__);              \
-  else if (s.nt == 64 && s.nch == 2) KERNEL(64, 2, __VA_ARGS__);              \
-  else if (s.nt == 64) KERNEL(64, 3, __VA_ARGS__);                            \
   else if (s.nt == 128) KERNEL(128, 1, __VA_ARGS__);                          \
   else if (s.nt == 256 && s.nch == 1) KERNEL(256, 1, __VA_ARGS__);            \
-  else if (s.nt == 256) KERNEL(256, 2, __VA_ARGS__);                          \
-  else if (s.nch == 1) KERNEL(512, 1, __VA_ARGS__);                           \
-  else KERNEL(512, 2, __VA_ARGS__)
+  else if (s.nt == 512 && s.nch == 1) KERNEL(512, 1, __VA_ARGS__);            \
+  else if (s.nt == 512) KERNEL(512, 2, __VA_ARGS__);                          \
+  else if constexpr (MANY) {                                                  \
+    if (s.nt == 64 && s.nch == 2) KERNEL(64, 2, __VA_ARGS__);                 \
+    else if (s.nt == 64) KERNEL(64, 3, __VA_ARGS__);                          \
+    else KERNEL(256, 2, __VA_ARGS__);                                         \
+  }
 
 template <int T>
 void launch_fwd(const LnArgs& a, int64_t B, hipStream_t st) {
@@ -423,9 +426,9 @@ void launch_fwd(const LnArgs& a, int64_t B, hipStream_t st) {
   }
 #define LN_F(NT, N, FULL) hipLaunchKernelGGL((ln_fwd_kernel<T, NT, N, FULL>), grid, dim3(64 * WAVES), 0, st, a)
   if (a.D % 8 == 0) {
-    LN_DISPATCH(LN_F, true);
+    LN_DISPATCH(LN_F, T < 2, true)
   } else {
-    LN_DISPATCH(LN_F, false);
+    LN_DISPATCH(LN_F, false, false)
   }
 #undef LN_F
 }
@@ -454,14 +457,14 @@ void launch_bwd(LnArgs a, int64_t B, hipStream_t st) {
     if (pg) hipLaunchKernelGGL((ln_wide_param_kernel<T>), dim3((a.D + 2047) / 2048, (unsigned)np, (unsigned)B), dim3(256), 0, st, a);
   } else if (pg && !fold) {
     if (a.D % 8 == 0) {
-      LN_DISPATCH(LN_B, true, true);
+      LN_DISPATCH(LN_B, false, true, true)
     } else {
-      LN_DISPATCH(LN_B, false, true);
+      LN_DISPATCH(LN_B, false, false, true)
     }
   } else if (a.D % 8 == 0) {
-    LN_DISPATCH(LN_B, true, false);
+    LN_DISPATCH(LN_B, T < 2, true, false)
   } else {
-    LN_DISPATCH(LN_B, false, false);
+    LN_DISPATCH(LN_B, false, false, false)
   }
 #undef LN_B
   if (pg && !fold && !a.direct) {

@@ -24,7 +24,7 @@ struct RopeArgs {
   const void* pos;
   const double* freq;
   int64_t pb, pt, ntok;                // element strides of the positions; B * T
-  int pos64, n_axes, ax1, ax2, ax3;    // first pair of axis 1, 2, 3
+  int pos64, ax1, ax2, ax3;            // first pair of axis 1, 2, 3
   int T, H, K, hd, rot, tb, slots, lanes;
   uint32_t magic;                      // ceil(2^32 / heads): i / heads = umulhi(i, magic) for i heads < 2^32
   float scale;
@@ -277,7 +277,7 @@ extern "C" int fluxhip_rotary(const fluxhip_rotary_desc* d, void* stream) {
   a.q = {d->q, d->q_out, d->q_strides[0], d->q_strides[1], d->q_strides[2], d->qo_strides[0], d->qo_strides[1], d->qo_strides[2]};
   a.k = {d->k, d->k_out, d->k_strides[0], d->k_strides[1], d->k_strides[2], d->ko_strides[0], d->ko_strides[1], d->ko_strides[2]};
   a.pos = d->positions; a.freq = (const double*)d->freqs;
-  a.pb = d->pos_strides[0]; a.pt = d->pos_strides[1]; a.pos64 = d->pos64; a.n_axes = d->n_axes;
+  a.pb = d->pos_strides[0]; a.pt = d->pos_strides[1]; a.pos64 = d->pos64;
   a.ax1 = ax[1]; a.ax2 = ax[2]; a.ax3 = ax[3];
   a.ntok = ntok; a.T = (int)d->T; a.H = d->H; a.K = d->K; a.hd = d->hd; a.rot = d->rot; a.scale = d->scale;
   const int part = d->interleaved ? d->rot : d->rot / 2, tail = d->hd - d->rot, V = d->dtype == 2 ? 4 : 8;

@@ -59,6 +59,30 @@ def test_layernorm_infinities_stay_in_their_row_and_column(dev, T, D, per, dt):
         assert bool(hg.view(-1, D)[-1].isnan().all()) and torch.equal(hg.view(-1, D)[:-1], gg.view(-1, D)[:-1])
 
 
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("per", [False, True])
+@pytest.mark.parametrize("T,D", [(2100, 640), (2048, 1024), (2049, 1032), (2300, 1536), (2050, 2056), (2048, 2560), (2047, 640), (2047, 2560)])
+def test_layernorm_of_many_rows_at_every_chunk_count(dev, T, D, per, dt):
+    """From 2048 rows on, 16-bit rows of whole chunks have two or three chunks a lane in the forward pass and in dx alone."""
+    from flux_generator_amd import ops
+    B, off = (2, 1.0) if per else (1, 0.0)
+    T //= B
+    x, dy = rnd(B, T, D, mean=0.5, seed=1, dt=dt), rnd(B, T, D, seed=2, dt=dt)
+    shape = (B, D) if per else (D,)
+    g, b = rnd(*shape, scale=0.3, mean=1 - off, seed=3, dt=dt), rnd(*shape, scale=0.3, seed=4, dt=dt)
+    c = lambda t: t.to(dev)
+    y, mu, r = ops.layernorm(c(x), c(g), c(b), unit_offset=per)
+    gd, bd = D64(g).reshape(-1, 1, D), D64(b).reshape(-1, 1, D)
+    for what, got, pair in zip(("y", "mean", "rstd"), (y, mu, r), R.ln_forward_bound(D64(x), gd, bd, 1e-5, off, dt)):
+        R.check(got, pair, what)
+    pairs = R.ln_backward_bound(D64(dy), D64(x), D64(mu), D64(r), gd, off, dt, dt, per)
+    for what, got, pair in zip(("dx", "dgamma", "dbeta"), ops.layernorm_backward(c(dy), c(x), mu, r, c(g), unit_offset=per), pairs):
+        R.check(got, pair, what)
+    R.check(ops.layernorm_backward(c(dy), c(x), mu, r, c(g), unit_offset=per, param_grads=False)[0], pairs[0], "dx alone")
+    R.check(ops.layernorm_backward(c(dy), c(x), mu, r)[0], R.ln_backward_bound(D64(dy), D64(x), D64(mu), D64(r), torch.ones(1, 1, D).double(), 0.0, dt, dt, False)[0],
+            "dx without parameters")
+
+
 # ------------------------------------------------------------------------------------------------ gated feed-forward
 @pytest.mark.parametrize("kind,name", [("erf", "EPI_GELU_ERF"), ("tanh", "EPI_GELU_TANH"), ("silu", "EPI_SILU")])
 @pytest.mark.parametrize("dt", [BF, HF])
