@@ -4,11 +4,16 @@
 //   dh = dy Wo, dvalue = dh act(gate), dgate = dh value act'(gate)
 //   dx = dvalue Wv + dgate Wg, dWv = dvalue^T x, dWg = dgate^T x, dWo = dy^T hidden, db = column sums
 //
-// Five matrix products of 2 M D F flops each way and more (6 M D F forward, 12 M D F backward): MFMA-bound for many tokens, bound
-// by the bytes of the weights for few.  One kernel template serves them: out[m][n] = sum_k Q(m, k) P(n, k), where either operand
+// Three matrix products of 2 M D F flops forward, six backward (three with frozen weights): MFMA-bound for many tokens, bound by the
+// bytes of the weights for few.  One kernel template serves them: out[m][n] = sum_k Q(m, k) P(n, k), where either operand
 // lies with k contiguous ("row": activations and nn.Linear weights in the forward pass) or with k strided ("col": the weights of
 // the input gradient, both operands of the weight gradients).  Nothing is transposed in memory: a "col" tile is staged as it lies
 // and its fragments are read with the transposing LDS read of this chip (ds_read_b64_tr_b16).
+//
+// Roundings: products and column sums accumulate in float32.  hidden, dvalue and dgate are rounded to the tensors' type before the
+// next product, whose MFMA takes 16-bit operands (a second MFMA for a low half would double that product); hidden is formed from the
+// unrounded value and gate.  What lies behind such an operand ends 1.4 roundings from the exact result instead of one (bf16 2.3e-3
+// against 1.7e-3).
 //
 // P is the MFMA's first operand, so a lane's four accumulators are four neighbouring n of one m; one permlane16 swap per register
 // pair makes that eight (a 16-byte store).
@@ -237,7 +242,7 @@ DEVINL Item item_of(const FfArgs& a, int it) {
 }
 
 // writes J m fragments of a wave's tile, from the j0-th.  Rows outside, their columns inside: one row's pieces (of one or several
-// tensors) are written together, which keeps the pages in reach of the CU's TLB (dvalue / dgate of 16384 x 5120: 372 -> 325 us
+// tensors) are written together, which keeps the pages in reach of the CU's TLB (dvalue / dgate of 16384 x 5120 from 1280: 372 -> 325 us
 // against the other order), and pairs of fragments are traded into whole 128-byte lines (from 128: 200 -> 163 us; a plain copy in
 // that tiling: 157 -> 140).
 template <int NF, int EPI, bool H, int J>
@@ -341,8 +346,10 @@ DEVINL void epilogue(const FfArgs& a, const FfProd& pr, f32x4 (&acc)[NF][J], int
     }
   } else if constexpr (EPI == EPI_DH) {
     // The saved value and gate of the next 16 rows are in flight while these are worked on (large tiles: from the middle of the
-    // work, where registers are free - 16384 x 5120 from 1280 298 us, 314 with 94 spilled registers from its start; small ones
-    // 163 / 168 from 128).  64 columns a pass, whose sums fit the registers.
+    // work, where registers are free - on repeated operands and without bias sums 16384 x 5120 from 1280 took 298 us, from its
+    // start 314 with 94 spilled registers; small ones 163 / 168 from 128.  On changing operands 312, with bias sums 325.)  The
+    // large kernel stands at 256 registers and still spills 11 (bf16) or 17 (f16) of them.  64 columns a pass, whose sums fit the
+    // registers.
     constexpr int PASS = 2;
     static_assert(HALVES % PASS == 0, "whole lines");
     const auto value = rows_of(a.value), gate = rows_of(a.gate), vout = rows_of(a.vout), gout = rows_of(a.gout);
@@ -568,7 +575,8 @@ __global__ __launch_bounds__(NF == 4 ? 256 : 512, 2) void ff_gemm_kernel(FfArgs 
 }
 
 // adds a split tile's partials in split order and writes it; a block takes one m fragment of each wave's tile.  Few blocks where few
-// rows are: bound by latency, so four splits' loads are in flight (forward of 36 tokens, 1064 -> 240: 16.5 us, with two 21.2)
+// rows are: bound by latency, so four splits' loads are in flight (forward of 36 tokens, 1064 -> 240, on repeated operands: 16.5 us, with
+// two 21.2; on changing ones 18.8, 6.4 of them here)
 template <int NF, int EPI, bool H>
 __global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a) {
   typedef Geo<NF, EPI> G;
@@ -591,8 +599,8 @@ __global__ __launch_bounds__(NF == 4 ? 256 : 512) void ff_finish_kernel(FfArgs a
 
 // ---- one or two tokens (serving): bound by reading the weights once.  A wave owns one output column - its value and gate row, or
 // its row of the out weight - and reads the rows whole, 1 KiB at a time and eight loads ahead, against the tokens' vectors from
-// L1; products are float32 FMAs.  4096 -> 10240 at one token: 26.8 us for 168 MB (6.3 TB/s), back 15.5 us.  (Three tokens and
-// more: the tiles above with their split along k are faster: 56 us forward at four tokens, 90 this way.)
+// L1; products are float32 FMAs.  4096 -> 10240 at one token: 26.0 us for 168 MB (6.4 TB/s), back 15.4 us.  (Three tokens and
+// more: the tiles above with their split along k are faster: 63 us forward at four tokens, 90 this way.)
 constexpr int GEMV = 2;
 template <bool DUAL, int MT, bool H>
 __global__ __launch_bounds__(256) void ff_gemv_kernel(FfArgs a) {
@@ -681,11 +689,13 @@ __global__ __launch_bounds__(64) void ff_colsum_kernel(const uint16_t* x, int64_
 // How a launch is cut: the estimated time of every way, the least wins.  256-square tiles run one block a CU at 1.5 us a step (64 k)
 // of all CUs, 128-square ones two a CU at 1.13 us (16384 x 5120 x 1280 and 512 x 20480 x 4096, bf16).  What the epilogue moves
 // comes on top at 4.9 TB/s - all of it for the large tiles, whose CU has nothing else to run, a bit more than half for the small
-// ones (dvalue / dgate of 16384 x 5120: from 128 178 / 163 us, from 1280 298 / 341).  Whole rounds of tiles run
-// as they are; the tiles of the last, broken round are split along k over the idle CUs where that pays for writing and reading
-// their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 8 us for the second launch).
+// ones (dvalue / dgate of 16384 x 5120 on repeated operands, large / small: from 128 178 / 163 us, from 1280 298 / 341).  Whole
+// rounds of tiles run as they are; the tiles of the last, broken round are split along k over the idle CUs where that pays for
+// writing and reading their float32 partials (0.117 us a 256-square split tile at 4.5 TB/s over the chip, and 8 us for the second
+// launch).
 // 256 x 192 tiles (row operands only; 1.2 us) where they fill the CUs better: EPI_UP of 512 x 10240 from 4096 is 214 of them in
-// 108 us, or 160 squares in 118; its product back, split, 59.6 and 9.8 adding up, with squares 51 and 15.
+// 96 to 109 us (the estimate says 81: it prices loops whose weights lie in the caches, these come from HBM), or 160 squares in 118;
+// its product back, split, 57 to 60 and 9.5 adding up, with squares 51 and 15.
 struct Plan { int nf, full, splits, items; };
 struct Dims { int64_t M, N; };                             // output of a product; EPI_UP: N = F
 int64_t tile_rows(int nf) { return nf == 4 ? 128 : 256; }
@@ -755,7 +765,7 @@ Plan plan_dw1(int64_t M, int D, int F) { const Dims d{D, F}; return pick(&d, 1, 
 int64_t colsum_rows(int64_t M, const Plan& p) {
   return (M + tile_rows(p.nf) - 1) / tile_rows(p.nf) * (tile_rows(p.nf) / 64) * (p.splits > 1 ? 4 : 1);
 }
-constexpr int COLSUM_ROWS = 1024;                          // (16384 x 1280, both stages: 15.1 us, with 512 17.4)
+constexpr int COLSUM_ROWS = 1024;                          // (16384 x 1280, both stages alone: 15.1 us, with 512 17.4)
 
 bool bad(int64_t M, int D, int F, int act, int dtype) {
   return M < 0 || M > (1 << 30) || D < 8 || F < 8 || D % 8 || F % 8 || D > (1 << 20) || F > (1 << 20) || dtype < 0 || dtype > 1 ||

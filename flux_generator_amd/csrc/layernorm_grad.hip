@@ -8,12 +8,12 @@
 // sample ([B][D], adaLN) - then the reduction of their gradient stops at the sample.  Row starts need only element alignment:
 // the 16-byte loads of this chip take any address, so an odd width costs its last chunk's element loads and nothing else.
 // The parameter gradient is a two-stage sum in a fixed order: every block adds its rows' contributions in registers and
-// writes one float32 partial row, ln_partial_sum_kernel adds those; no atomics, so the result is the same in every run.
+// writes one float32 partial row, colsum_final_kernel (colsum.h) adds those; no atomics, so the result is the same in every run.
+// (Rows are added one after the other: float32 gradients of 231 rows end 1.2e-7 from the exact ones, with pairwise sums 0.9e-7.)
 #include "../../include/fluxhip.h"
 #include "common.h"
 #include "elem.h"
 #include "colsum.h"
-
 
 namespace {
 
@@ -367,9 +367,9 @@ __global__ __launch_bounds__(256) void ln_wide_param_kernel(LnArgs a) {
 
 // Threads per row and chunks per thread.  Few rows, float32, a parameter gradient or a width that cuts a chunk: as many threads as
 // have one chunk each - short serial work, and registers stay free for the loads in flight.  Else two or three chunks a lane, which
-// leaves fewer idle lanes and fewer barriers.  Measured (us, several chunks / one): 16384 x 1280 f16 forward 20.2 / 23.4, dx alone
-// 24.1 / 24.8, with parameter gradient 45.4 / 42.2; 4 x 4096 x 2560 bf16 36.4 / 40.6, 41.8 / 43.1, 59.0 / 52.9; 16384 x 1280
-// float32 32.3 / 30.1, 62.9 / 41.7, 62.8 / 55.6.
+// leaves fewer idle lanes and fewer barriers.  Measured (us a call on changing operands, several chunks / one): 16384 x 1280 f16
+// forward 19.4 / 23.4, dx alone 24.6 / 26.9, with parameter gradient 37.0 / 34.2; 4 x 4096 x 2560 bf16 33.7 / 40.2, 42.3 / 51.9,
+// 60.5 / 53.9; 16384 x 1280 float32 32.2 / 30.1, 60.9 / 41.4, 53.7 / 46.5.
 struct Shape { int nt, nch; };
 Shape pick(int64_t rows, int D, bool f32, bool pg) {
   const int c = (D + 7) / 8;

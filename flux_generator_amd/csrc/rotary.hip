@@ -5,9 +5,10 @@
 // (interleaved) or (j, j + rot / 2) (half); the columns behind rot are copied.  HBM-bound: each element is read and written once.
 //
 // The angle is formed in 64 bits - at position 10^6 a float32 product is off by 0.06 rad - and reduced to a fraction of a turn
-// there; cos / sin of the fraction are float32.  A block takes TB consecutive tokens: one thread per (token, pair) computes the
-// pair's cos and sin ONCE into LDS, then all threads walk the tokens' q and k heads in vectors of V elements; a thread keeps its
-// columns and moves over (token, head) items.
+// there; cos / sin of the fraction are float32 (its rounding is at most 2 pi 2^-26 rad: a float32 result ends 4.7e-8 from the exact
+// one, with 64-bit sines 3.5e-8; 16-bit results do not see it).  A block takes TB consecutive tokens: one thread per (token, pair)
+// computes the pair's cos and sin ONCE into LDS, then all threads walk the tokens' q and k heads in vectors of V elements; a thread
+// keeps its columns and moves over (token, head) items.
 #include "../../include/fluxhip.h"
 #include "common.h"
 #include "elem.h"

@@ -1175,10 +1175,10 @@ def _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, inverse, out):
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, axes_dim=None,
            interleaved: bool = True, scale: float = 1.0, out=None):
     """Rotary positions on q [B, T, H, head_dim] and k [B, T, K, head_dim] (or None) in one launch -> (q', k') (or q').  Any strides
-    with a contiguous last dimension (transposed heads, slices of a fused projection); out: tensors to write, which may be q and k
-    themselves but are refused unless they provably lie apart from them otherwise.  positions [T] or [B, T] integers, with axes_dim of several axes [T, axes] or [B, T, axes]; freqs, scale:
-    rotary_frequencies.  The first 2 len(freqs) columns turn - pairs (2j, 2j + 1) when interleaved, else (j, j + half) -, the rest is
-    copied.  Angles are formed in 64 bits."""
+    with a contiguous last dimension (transposed heads, slices of a fused projection).  out: tensors to write - q and k themselves,
+    or tensors that provably lie apart from them and from each other; anything else is refused.  positions [T] or [B, T] integers,
+    with axes_dim of several axes [T, axes] or [B, T, axes]; freqs, scale: rotary_frequencies.  The first 2 len(freqs) columns turn
+    - pairs (2j, 2j + 1) when interleaved, else (j, j + half) -, the rest is copied.  Angles are formed in 64 bits."""
     return _rotary(q, k, positions, freqs, axes_dim, interleaved, scale, False, out)
 
 

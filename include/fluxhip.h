@@ -547,10 +547,10 @@ int fluxhip_layernorm_grad(const void* dy, int64_t dy_bs, int64_t dy_rs, const v
                            int64_t ws_bytes, void* stream);
 
 /* Rotary positions on q [B][T][H][hd] and k [B][T][K][hd] (element strides of batch, token, head; the last dimension is
- * contiguous; out may be in, but must not overlap it otherwise).  Pair j < rot / 2 of a token turns by positions[.., axis(j)] * freqs[j] (formed in 64 bits) and is
- * scaled by `scale`; columns >= rot are copied.  interleaved: pairs (2j, 2j + 1), else (j, j + rot / 2).  Axis i owns
- * axis_pairs[i] consecutive pairs (their sum is rot / 2).  inverse: the turn by the negative angle = the gradient.
- * flux/layers.py:29-33,60-75 in general form. */
+ * contiguous; an output may be its input, but overlaps no input or output otherwise).  Pair j < rot / 2 of a token turns by
+ * positions[.., axis(j)] * freqs[j] (formed in 64 bits) and is scaled by `scale`; columns >= rot are copied.  interleaved: pairs
+ * (2j, 2j + 1), else (j, j + rot / 2).  Axis i owns axis_pairs[i] consecutive pairs (their sum is rot / 2).  inverse: the turn by the
+ * negative angle = the gradient.  flux/layers.py:29-33,60-75 in general form. */
 typedef struct fluxhip_rotary_desc {
   const void *q, *k;
   void *q_out, *k_out;
